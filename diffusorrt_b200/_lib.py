@@ -34,6 +34,11 @@ SELECT_MAX_PROB = 0
 SELECT_NEG_ENTROPY = 1
 TIE_NEAR = 1
 TIE_EXACT = 2
+CODE_INT8 = 0
+CODE_E4M3 = 1
+TYPE_F32 = 0
+TYPE_BF16 = 1
+TYPE_F16 = 2
 
 
 class DrtError(RuntimeError):
@@ -96,7 +101,20 @@ class Metrics(ctypes.Structure):
                 ("device_bytes", ctypes.c_int64)]
 
 
+class CacheAttendArgs(ctypes.Structure):
+    _fields_ = ([("q", ctypes.c_void_p), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64), ("out", ctypes.c_void_p),
+                 ("out_row", ctypes.c_int64), ("out_head", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("lse", "k_cache", "v_cache", "k_scale", "v_scale")]
+                + [("blocks", ctypes.c_int64), ("tables", ctypes.c_void_p), ("ld_tables", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("lengths", "row_start", "origin", "scratch")]
+                + [(n, ctypes.c_int32) for n in ("q_rows", "heads", "kv_heads", "dim", "dtype", "code", "block", "width",
+                                                 "requests", "mask_block", "max_rows")]
+                + [("scale", ctypes.c_float)])
+
+
 _P = ctypes.c_void_p
+_I32 = ctypes.c_int32
+_I64 = ctypes.c_int64
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _F64P = ctypes.POINTER(ctypes.c_double)
 
@@ -158,6 +176,16 @@ SIGNATURES = {
     "drt_quantize_q8": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int32, _P, _P, _P, _P]),
     "drt_linear_q8": (ctypes.c_int, [_P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                      _P]),
+    "drt_cache_plan": (ctypes.c_int, [_P, _P, _P, _P, _I32, _P, _I64, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P, _I32, _P,
+                                      _P, _P]),
+    "drt_cache_append": (ctypes.c_int, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _P, _P, _I64, _I32, _I32,
+                                        _I32, _I32, _P]),
+    "drt_cache_read": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _P]),
+    "drt_cache_attend_scratch_bytes": (ctypes.c_size_t, [_I32]),
+    "drt_cache_attend": (ctypes.c_int, [ctypes.POINTER(CacheAttendArgs), _P]),
+    "drt_selector_logprobs_scratch_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
+    "drt_selector_logprobs": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I32, _P, ctypes.c_double, _I32, _I32, _P, _P, _P,
+                                             _P, _P, _P, _P]),
     "drt_linear_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     "drt_linear_bf16": (ctypes.c_int, [_P, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                        ctypes.c_int32, _P, _P]),

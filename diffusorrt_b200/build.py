@@ -13,8 +13,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libdiffusorrt_b200.so"
-SOURCES = [CSRC / "capi.cu"]
-HEADERS = sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "diffusorrt_b200.h"]
+SOURCES = [CSRC / "capi.cu", CSRC / "capi_serve.cu"]
+HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [PKG.parent / "include" / "diffusorrt_b200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -22,6 +22,7 @@
 #include "../../include/diffusorrt_b200.h"
 #include "attention.cuh"
 #include "attention_decode.cuh"
+#include "capi_common.h"
 #include "common.cuh"
 #include "dream.cuh"
 #include "gemm.cuh"
@@ -37,8 +38,9 @@ using namespace drt;
 // ======================================================================= errors
 namespace {
 thread_local std::string g_last_error;
+}  // namespace
 
-int set_error(int code, const char* fmt, ...) {
+int drt::set_error(int code, const char* fmt, ...) {
   char buf[1024];
   va_list ap;
   va_start(ap, fmt);
@@ -47,24 +49,6 @@ int set_error(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
-}  // namespace
-
-#define CK(expr)                                                                                         \
-  do {                                                                                                   \
-    cudaError_t _e = (expr);                                                                             \
-    if (_e != cudaSuccess)                                                                               \
-      return set_error(DRT_INTERNAL_ERROR, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(_e), __FILE__, \
-                       __LINE__);                                                                        \
-  } while (0)
-#define TRY(expr)                 \
-  do {                            \
-    int _r = (expr);              \
-    if (_r != DRT_OK) return _r;  \
-  } while (0)
-#define REQUIRE(cond, ...)                                     \
-  do {                                                         \
-    if (!(cond)) return set_error(DRT_INVALID_ARGUMENT, __VA_ARGS__); \
-  } while (0)
 
 // ======================================================================= TMA descriptors
 namespace {

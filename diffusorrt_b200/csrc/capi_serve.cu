@@ -1,0 +1,372 @@
+// C ABI of the batch-serving operators: the paged 8-bit K/V cache (block tables, append, read back,
+// attention) and the token scorer. Device pointers and a stream from the caller, no allocation.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstring>
+
+#include "attention_q8.cuh"
+#include "capi_common.h"
+#include "kvcache.cuh"
+#include "logprobs.cuh"
+
+using namespace drt;
+
+namespace {
+
+template <typename... P, typename... Args>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl ? attr : nullptr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// SM count of the current device; 0 with an error recorded.
+int current_sms(int* device) {
+  static std::atomic<int> cache[64];
+  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= 64) return 0;
+  int n = cache[*device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) != cudaSuccess) return 0;
+    cache[*device].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Allows Kernel its dynamic shared memory on the current device (the attribute is per device).
+template <auto Kernel>
+cudaError_t allow_smem(int device, size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  if (done.load(std::memory_order_acquire) >> device & 1) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) done.fetch_or(1ull << device, std::memory_order_release);
+  return e;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool block_ok(int b) { return b == 16 || b == 32 || b == 64 || b == 128; }
+
+}  // namespace
+
+// ======================================================================= block tables and slot maps
+extern "C" int drt_cache_plan(const int32_t* start, const int32_t* count, const int32_t* held_in, int32_t* held_out,
+                              int32_t requests, int32_t* tables, int64_t ld_tables, int32_t width, int32_t block,
+                              int32_t* ring, int32_t ring_size, const int32_t* ring_in, int32_t* ring_out,
+                              int32_t* row_start, int32_t* slots, int32_t* positions, int32_t max_rows, int32_t* lengths,
+                              int32_t* status, void* stream) {
+  REQUIRE(requests >= 0 && requests <= (1 << 20), "requests outside [0, 2^20]");
+  REQUIRE(row_start && ring && ring_in && ring_out && status, "null argument");
+  REQUIRE(requests == 0 || (start && count && held_in && held_out && tables && lengths), "null argument");
+  REQUIRE(max_rows >= 0 && (max_rows == 0 || (slots && positions)), "max_rows needs slots and positions");
+  REQUIRE(block >= 1 && width >= 1 && ld_tables >= width, "bad table geometry");
+  REQUIRE(static_cast<int64_t>(width) * block <= INT32_MAX, "a request's tokens exceed 2^31 - 1");
+  REQUIRE(ring_size >= 1, "the ring needs a capacity");
+  PlanArgs a;
+  memset(&a, 0, sizeof(a));
+  a.start = start;
+  a.count = count;
+  a.held_in = held_in;
+  a.held_out = held_out;
+  a.requests = requests;
+  a.tables = tables;
+  a.ld_tables = ld_tables;
+  a.width = width;
+  a.block = block;
+  a.ring = ring;
+  a.ring_size = ring_size;
+  a.ring_in = ring_in;
+  a.ring_out = ring_out;
+  a.row_start = row_start;
+  a.slots = slots;
+  a.positions = positions;
+  a.max_rows = max_rows;
+  a.lengths = lengths;
+  a.status = status;
+  a.fill_slots = max_rows <= kPlanInlineRows;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CK(launch(plan_cache_kernel, dim3(1), dim3(kPlanThreads), 0, st, false, a));
+  if (!a.fill_slots)
+    CK(launch(plan_slots_kernel, dim3((max_rows + kPlanSlotRows - 1) / kPlanSlotRows), dim3(256), 0, st, true, a));
+  return DRT_OK;
+}
+
+// ======================================================================= append and read back
+namespace {
+int check_cache(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, int64_t blocks,
+                int32_t heads, int32_t block, int32_t dim, int32_t code) {
+  REQUIRE(k_cache && v_cache && k_scale && v_scale, "null argument");
+  REQUIRE(blocks >= 1 && heads >= 1 && heads <= 65535, "bad cache geometry");
+  REQUIRE(block_ok(block), "a block holds 16, 32, 64 or 128 tokens (got %d)", block);
+  REQUIRE(blocks * block <= INT32_MAX, "slots exceed 2^31 - 1");
+  if (dim != 64 && dim != 128) return set_error(DRT_UNSUPPORTED, "head dim %d: 64 and 128 are served", dim);
+  REQUIRE(code == DRT_CODE_INT8 || code == DRT_CODE_E4M3, "unknown code type %d", code);
+  REQUIRE(aligned16(k_cache) && aligned16(v_cache), "the caches must be 16-byte aligned");
+  return DRT_OK;
+}
+
+template <typename T, int kDim, int kCode>
+cudaError_t run_append(const AppendArgs& a, cudaStream_t st) {
+  return launch(append_cache_kernel<T, kDim, kCode>, dim3((a.rows + a.group - 1) / a.group, a.heads, 2), dim3(kAppendThreads),
+                0, st, false, a);
+}
+template <typename T, int kDim, int kCode>
+cudaError_t run_read(const ReadArgs& a, cudaStream_t st) {
+  return launch(read_cache_kernel<T, kDim, kCode>, dim3((a.rows + kReadRows - 1) / kReadRows, a.heads), dim3(kReadThreads), 0,
+                st, false, a);
+}
+}  // namespace
+
+#define DRT_DISPATCH_DIM_CODE(fn, T, ...)                                                      \
+  (dim == 128 ? (code == DRT_CODE_INT8 ? fn<T, 128, CACHE_INT8>(__VA_ARGS__) : fn<T, 128, CACHE_E4M3>(__VA_ARGS__)) \
+              : (code == DRT_CODE_INT8 ? fn<T, 64, CACHE_INT8>(__VA_ARGS__) : fn<T, 64, CACHE_E4M3>(__VA_ARGS__)))
+
+extern "C" int drt_cache_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                                int32_t dtype, int32_t rows, const int32_t* slots, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, int64_t blocks, int32_t heads, int32_t block, int32_t dim,
+                                int32_t code, void* stream) {
+  REQUIRE(rows >= 0, "rows must be >= 0");
+  TRY(check_cache(k_cache, v_cache, k_scale, v_scale, blocks, heads, block, dim, code));
+  REQUIRE(dtype == DRT_TYPE_BF16 || dtype == DRT_TYPE_F16, "k and v must be bf16 or f16");
+  if (rows == 0) return DRT_OK;
+  REQUIRE(k && v && slots, "null argument");
+  AppendArgs a;
+  memset(&a, 0, sizeof(a));
+  a.k = k;
+  a.v = v;
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.slots = slots;
+  a.rows = rows;
+  a.heads = heads;
+  a.block = block;
+  a.group = rows <= kAppendSingleRows ? 1 : 16;
+  a.blocks = blocks;
+  a.k_cache = static_cast<uint8_t*>(k_cache);
+  a.v_cache = static_cast<uint8_t*>(v_cache);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.vec = aligned16(k) && aligned16(v) && (k_row | k_head | v_row | v_head) % 8 == 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CK(dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_append, __nv_bfloat16, a, st)
+                            : DRT_DISPATCH_DIM_CODE(run_append, __half, a, st));
+  return DRT_OK;
+}
+
+extern "C" int drt_cache_read(const int32_t* slots, int32_t rows, const void* k_cache, const void* v_cache,
+                              const float* k_scale, const float* v_scale, int64_t blocks, int32_t heads, int32_t block,
+                              int32_t dim, int32_t code, void* k_out, void* v_out, int32_t dtype, void* stream) {
+  REQUIRE(rows >= 0, "rows must be >= 0");
+  TRY(check_cache(k_cache, v_cache, k_scale, v_scale, blocks, heads, block, dim, code));
+  REQUIRE(dtype == DRT_TYPE_BF16 || dtype == DRT_TYPE_F16 || dtype == DRT_TYPE_F32, "values are read as bf16, f16 or f32");
+  if (rows == 0) return DRT_OK;
+  REQUIRE(slots && k_out && v_out, "null argument");
+  REQUIRE(aligned16(k_out) && aligned16(v_out), "the outputs must be 16-byte aligned");
+  ReadArgs a;
+  memset(&a, 0, sizeof(a));
+  a.slots = slots;
+  a.rows = rows;
+  a.heads = heads;
+  a.block = block;
+  a.blocks = blocks;
+  a.k_cache = static_cast<const uint8_t*>(k_cache);
+  a.v_cache = static_cast<const uint8_t*>(v_cache);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CK(dtype == DRT_TYPE_BF16  ? DRT_DISPATCH_DIM_CODE(run_read, __nv_bfloat16, a, st)
+     : dtype == DRT_TYPE_F16 ? DRT_DISPATCH_DIM_CODE(run_read, __half, a, st)
+                             : DRT_DISPATCH_DIM_CODE(run_read, float, a, st));
+  return DRT_OK;
+}
+
+// ======================================================================= attention over the cache
+namespace {
+constexpr size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// Scratch of a call: partial sums, their statistics and the cut units' descriptors, for every share.
+size_t attend_bytes(int shares, int tile_rows, int dim) {
+  return up256(static_cast<size_t>(shares) * 2 * tile_rows * dim * 4) + up256(static_cast<size_t>(shares) * 2 * tile_rows * 16) +
+         up256(static_cast<size_t>(shares) * 2 * 16);
+}
+
+template <typename T, int kDim, int kCode>
+cudaError_t run_rows(const CacheAttnArgs& a, int device, int grid, int merge_rows, cudaStream_t st) {
+  const size_t smem = QrCfg<kDim>::kSmem;
+  cudaError_t e = allow_smem<cache_attn_rows_kernel<T, kDim, kCode>>(device, smem);
+  if (e == cudaSuccess) e = launch(cache_attn_rows_kernel<T, kDim, kCode>, dim3(grid), dim3(kQrThreads), smem, st, false, a);
+  if (e != cudaSuccess || merge_rows == 0) return e;
+  const int shares = grid * kQrWarps;
+  return launch(cache_attn_merge_kernel<T, kDim, kQrRows>, dim3((shares + kQmWarps - 1) / kQmWarps, merge_rows),
+                dim3(kQmThreads), 0, st, true, a, shares);
+}
+}  // namespace
+
+extern "C" size_t drt_cache_attend_scratch_bytes(int32_t dim) {
+  int device = 0;
+  const int sms = current_sms(&device);
+  return attend_bytes((sms > 0 ? sms : 148) * kQrWarps, kQrRows, dim);
+}
+
+extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
+  REQUIRE(p, "null argument");
+  TRY(check_cache(p->k_cache, p->v_cache, p->k_scale, p->v_scale, p->blocks, p->kv_heads, p->block, p->dim, p->code));
+  REQUIRE(p->dtype == DRT_TYPE_BF16 || p->dtype == DRT_TYPE_F16, "q and out must be bf16 or f16");
+  REQUIRE(p->heads >= 1 && p->heads % p->kv_heads == 0, "query heads must be a multiple of the K/V heads");
+  REQUIRE(p->q_rows >= 0 && p->requests >= 0 && p->requests <= kQrMaxRequests, "requests outside [0, %d]", kQrMaxRequests);
+  REQUIRE(static_cast<int64_t>(p->q_rows) * p->heads <= INT32_MAX, "rows times heads exceed 2^31 - 1");
+  REQUIRE(p->width >= 1 && p->ld_tables >= p->width && static_cast<int64_t>(p->width) * p->block <= INT32_MAX,
+          "bad table geometry");
+  REQUIRE(p->mask_block >= 0 && p->mask_block <= (1 << 24), "mask_block outside [0, 2^24]");
+  REQUIRE(std::isfinite(p->scale) && p->scale >= 0.0f, "scale must be finite and >= 0");
+  if (p->q_rows == 0 || p->requests == 0) return DRT_OK;
+  REQUIRE(p->q && p->out && p->tables && p->lengths && p->row_start && p->scratch, "null argument");
+  REQUIRE(reinterpret_cast<uintptr_t>(p->out) % 4 == 0 && (p->out_row | p->out_head) % 2 == 0, "out rows must be 4-byte aligned");
+  REQUIRE(aligned16(p->scratch), "scratch must be 16-byte aligned");
+  int device = 0;
+  const int sms = current_sms(&device);
+  if (sms == 0) return set_error(DRT_INTERNAL_ERROR, "no current CUDA device");
+  CacheAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = p->q;
+  a.q_row = p->q_row;
+  a.q_head = p->q_head;
+  a.q_rows = p->q_rows;
+  a.k_cache = static_cast<const uint8_t*>(p->k_cache);
+  a.v_cache = static_cast<const uint8_t*>(p->v_cache);
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.blocks = p->blocks;
+  a.block = p->block;
+  a.heads = p->kv_heads;
+  a.group = p->heads / p->kv_heads;
+  a.tables = p->tables;
+  a.ld_tables = p->ld_tables;
+  a.width = p->width;
+  a.lengths = p->lengths;
+  a.row_start = p->row_start;
+  a.origin = p->origin;
+  a.requests = p->requests;
+  a.mask_block = p->mask_block;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.out = p->out;
+  a.out_row = p->out_row;
+  a.out_head = p->out_head;
+  a.lse = p->lse;
+  a.vec = aligned16(p->q) && (p->q_row | p->q_head) % 8 == 0;
+  const int shares = sms * kQrWarps;
+  uint8_t* s = static_cast<uint8_t*>(p->scratch);
+  a.part = reinterpret_cast<float*>(s);
+  s += up256(static_cast<size_t>(shares) * 2 * kQrRows * p->dim * 4);
+  a.stat = reinterpret_cast<float4*>(s);
+  s += up256(static_cast<size_t>(shares) * 2 * kQrRows * 16);
+  a.desc = reinterpret_cast<int4*>(s);
+  const int max_rows = p->max_rows > 0 ? std::min(p->max_rows, p->q_rows) : p->q_rows;
+  // A unit's key tiles at most: with one there is nothing to cut and nothing to join.
+  const int64_t deep = (static_cast<int64_t>(p->width) * p->block + kQrTile - 1) / kQrTile;
+  const int64_t units = (static_cast<int64_t>(p->q_rows) * a.group / kQrRows + p->requests) * a.heads;
+  const int grid = static_cast<int>(std::min<int64_t>(sms, units * deep));
+  const int merge_rows = deep > 1 ? static_cast<int>(std::min<int64_t>(kQrRows, static_cast<int64_t>(max_rows) * a.group)) : 0;
+  const int dim = p->dim, code = p->code;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CK(p->dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_rows, __nv_bfloat16, a, device, grid, merge_rows, st)
+                               : DRT_DISPATCH_DIM_CODE(run_rows, __half, a, device, grid, merge_rows, st));
+  return DRT_OK;
+}
+
+// ======================================================================= token scores
+namespace {
+struct LpPlan {
+  int segs, slices, per;
+};
+LpPlan logprob_plan(int rows, int vocab, int type, int sms) {
+  const int elem = type == LOGIT_F32 ? 4 : 2;
+  const int seg = 4096 / elem;
+  LpPlan p;
+  p.segs = (vocab + 16 / elem - 1 + seg - 1) / seg;  // a row may begin inside a 16-byte vector
+  const int64_t total = static_cast<int64_t>(p.segs) * rows;
+  const int64_t want = total / (static_cast<int64_t>(sms) * kLpCtasPerSm);
+  p.per = static_cast<int>(std::min<int64_t>(std::max<int64_t>(want, kLpWarps), kLpMaxSliceSegs));
+  p.per = std::min(p.per, p.segs);
+  p.slices = (p.segs + p.per - 1) / p.per;
+  p.per = (p.segs + p.slices - 1) / p.slices;
+  return p;
+}
+
+template <typename T>
+cudaError_t run_logprobs(const LogprobArgs& a, cudaStream_t st) {
+  cudaError_t e = launch(logprob_stats_kernel<T>, dim3(static_cast<unsigned>(a.rows) * a.slices), dim3(kLpThreads), 0, st, false, a);
+  if (e != cudaSuccess) return e;
+  const size_t smem = a.top > 0 ? kLpCands * 8 + static_cast<size_t>(a.segs) * 4 : 0;
+  return launch(logprob_finish_kernel<T>, dim3(a.rows), dim3(kLpThreads), smem, st, true, a);
+}
+}  // namespace
+
+extern "C" size_t drt_selector_logprobs_scratch_bytes(int32_t rows, int32_t vocab, int32_t dtype) {
+  if (rows <= 0 || vocab <= 0) return 0;
+  int device = 0;
+  const int sms = current_sms(&device);
+  const LpPlan p = logprob_plan(rows, vocab, dtype, sms > 0 ? sms : 148);
+  return up256(static_cast<size_t>(rows) * p.slices * 16) + up256(static_cast<size_t>(rows) * p.segs * 4);
+}
+
+extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, const int32_t* row_index, int32_t rows,
+                                     int32_t vocab, const int32_t* tokens, double temperature, int32_t exclude_token,
+                                     int32_t top, void* scratch, float* logprob, float* entropy, int32_t* rank,
+                                     int32_t* top_token, float* top_logprob, void* stream) {
+  REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab, "bad selector geometry");
+  REQUIRE(dtype == DRT_TYPE_F32 || dtype == DRT_TYPE_BF16 || dtype == DRT_TYPE_F16, "logits must be f32, bf16 or f16");
+  REQUIRE(top >= 0 && top <= kLpMaxTop, "top must be in [0, %d]", kLpMaxTop);
+  REQUIRE(std::isfinite(temperature), "temperature must be finite");
+  REQUIRE(exclude_token >= -1 && exclude_token < vocab, "exclude_token outside the vocabulary");
+  if (rows == 0) return DRT_OK;
+  REQUIRE(logits && scratch && (top == 0 || (top_token && top_logprob)), "null argument");
+  REQUIRE(tokens || (!logprob && !rank), "logprob and rank need tokens");
+  REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == DRT_TYPE_F32 ? 4 : 2) == 0 && aligned16(scratch),
+          "logits or scratch misaligned");
+  int device = 0;
+  const int sms = current_sms(&device);
+  if (sms == 0) return set_error(DRT_INTERNAL_ERROR, "no current CUDA device");
+  const LpPlan p = logprob_plan(rows, vocab, dtype, sms);
+  REQUIRE(p.segs <= kLpMaxSegs, "rows of at most %d logits", kLpMaxSegs * (dtype == DRT_TYPE_F32 ? 1024 : 2048) - 8);
+  REQUIRE(static_cast<int64_t>(rows) * p.slices <= INT32_MAX, "too many rows");
+  LogprobArgs a;
+  memset(&a, 0, sizeof(a));
+  a.logits = logits;
+  a.ld = ld;
+  a.row_index = row_index;
+  a.tokens = tokens;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.top = top;
+  a.exclude = exclude_token;
+  a.unit = temperature > 0.0 ? static_cast<float>(1.0 / temperature) : 1.0f;
+  a.segs = p.segs;
+  a.slices = p.slices;
+  a.segs_per_slice = p.per;
+  a.part = static_cast<float4*>(scratch);
+  a.seg_max = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + up256(static_cast<size_t>(rows) * p.slices * 16));
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.rank = rank;
+  a.top_token = top_token;
+  a.top_logprob = top_logprob;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CK(dtype == DRT_TYPE_F32    ? run_logprobs<float>(a, st)
+     : dtype == DRT_TYPE_BF16 ? run_logprobs<__nv_bfloat16>(a, st)
+                              : run_logprobs<__half>(a, st));
+  return DRT_OK;
+}

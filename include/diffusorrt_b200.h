@@ -358,6 +358,92 @@ int drt_select_choices(const double* conf, const int32_t* offsets, int32_t n_ite
  * on the GPU (other streams, other threads) race and must be serialized by the caller. */
 int drt_selector_rows_noalloc(const float* logits, int64_t ld, int32_t n_rows, int32_t vocab, int32_t mode,
                               double temperature, double* conf, int32_t* token, void* stream);
+/* ------------------------------------------------------------------ batch serving (device pointers)
+ * A paged 8-bit K/V cache shared by many requests, and the scores of given tokens. No counterpart in the
+ * reference, whose sessions hold one request each (python/src/edllm/backends/mlx_state_cache.py:51-603).
+ * A block holds `block` tokens (16, 32, 64 or 128) of every K/V head:
+ *   K codes [blocks][kv_heads][block][dim], V codes [blocks][kv_heads][block / 16][dim][16], dim 64 or 128,
+ *   k_scale / v_scale [blocks][kv_heads] f32 (>= 0), value = scale * code,
+ * int8 codes in [-127, 127] or finite float8 e4m3. A slot is block id * block + offset. */
+#define DRT_CODE_INT8 0
+#define DRT_CODE_E4M3 1
+#define DRT_TYPE_F32 0
+#define DRT_TYPE_BF16 1
+#define DRT_TYPE_F16 2
+/* Block tables and slot maps of a step from the requests' lengths, on the device. Request r has start[r]
+ * tokens and held_in[r] blocks (the first entries of tables[r], `width` long) and gets count[r] >= 0 rows at
+ * positions start[r] ..; blocks that this takes beyond the held ones come from the ring. count[r] = -1: the
+ * request has finished, and its blocks go back to the ring. The ring is a circular buffer of ring_size block
+ * ids: ring_in[1] free ones from index ring_in[0] on; ring_out is the same after the call. Both orders are
+ * the requests'. Blocks given back serve later calls only. held_out may be held_in, ring_out ring_in.
+ * Out: row_start [requests + 1] (rows packed in request order), lengths (start + count, 0 if finished),
+ * slots and positions [max_rows], -1 behind the last row. All or nothing: status[0] = 0, or
+ *   > 0: so many blocks are missing; -2: a request outgrows its table row; -3: more than max_rows rows;
+ *   -4: a negative start, a count below -1, a held count outside the table, a ring state outside the ring;
+ * then no table, ring or held count changes, row_start is all 0, slots are -1 and lengths are start.
+ * Calling it again with the same start and count takes no further blocks, so a window may be planned anew
+ * for each of its denoising steps. */
+int drt_cache_plan(const int32_t* start, const int32_t* count, const int32_t* held_in, int32_t* held_out,
+                   int32_t requests, int32_t* tables, int64_t ld_tables, int32_t width, int32_t block, int32_t* ring,
+                   int32_t ring_size, const int32_t* ring_in, int32_t* ring_out, int32_t* row_start, int32_t* slots,
+                   int32_t* positions, int32_t max_rows, int32_t* lengths, int32_t* status, void* stream);
+/* Rows of K and V (bf16 or f16 [rows][kv_heads][dim], strides in elements, dim contiguous) into the cache.
+ * Rows with consecutive slots of one block form a run; per run and head
+ *   s = max(amax / Q, the block's scale unless the run begins the block), Q = 127 or 448, code = rn(x / s);
+ * the block's other tokens are rounded anew when s has grown. A run that begins a block starts it anew: its
+ * earlier tokens and scale are gone. amax is over finite values; an infinity takes the largest code, a NaN 0.
+ * Slots outside the cache (-1) are skipped. Within a call the slots are distinct, and those of one block are
+ * one run (as drt_cache_plan gives them). */
+int drt_cache_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                     int32_t dtype, int32_t rows, const int32_t* slots, void* k_cache, void* v_cache, float* k_scale,
+                     float* v_scale, int64_t blocks, int32_t heads, int32_t block, int32_t dim, int32_t code,
+                     void* stream);
+/* The values scale * code of the listed slots, rounded once to dtype: k_out, v_out [rows][heads][dim]
+ * contiguous. A slot outside the cache gives zeros. */
+int drt_cache_read(const int32_t* slots, int32_t rows, const void* k_cache, const void* v_cache, const float* k_scale,
+                   const float* v_scale, int64_t blocks, int32_t heads, int32_t block, int32_t dim, int32_t code,
+                   void* k_out, void* v_out, int32_t dtype, void* stream);
+/* Attention of the rows of many requests over the cache. Row i of request r's n rows (row_start[r] + i in
+ * q and out) stands at position p = lengths[r] - n + i: its own token is in the cache already. It sees
+ *   mask_block b >= 1: keys below o + ((p - o) / b + 1) b with o = origin[r] (0 without origin), below o
+ *                      where p < o; b = 1 is causal, a block size gives the d2f_hybrid mask;
+ *   mask_block 0:      every key;
+ * never one at lengths[r] or behind. A row that sees nothing gets zeros and lse -inf; rows of out and lse
+ * behind row_start[requests] are left as they were. A table entry outside the cache hides its tokens. */
+typedef struct drt_cache_attend_args {
+  const void* q;              /* [q_rows][heads][dim], dtype DRT_TYPE_BF16 or _F16, dim contiguous */
+  int64_t q_row, q_head;      /* strides in elements */
+  void* out;                  /* as q, its own strides */
+  int64_t out_row, out_head;
+  float* lse;                 /* optional [q_rows][heads]: ln sum exp of the scaled scores */
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  int64_t blocks;
+  const int32_t* tables;      /* [requests][ld_tables], `width` entries used */
+  int64_t ld_tables;
+  const int32_t* lengths;     /* [requests] */
+  const int32_t* row_start;   /* [requests + 1] */
+  const int32_t* origin;      /* optional [requests] */
+  void* scratch;              /* drt_cache_attend_scratch_bytes(dim), one per call in flight */
+  int32_t q_rows, heads, kv_heads, dim, dtype, code, block, width, requests;
+  int32_t mask_block;
+  int32_t max_rows;           /* the caller's bound on a request's rows (0: q_rows); only chooses kernels */
+  float scale;                /* of the scores, usually 1 / sqrt(dim) */
+} drt_cache_attend_args;
+size_t drt_cache_attend_scratch_bytes(int32_t dim);
+int drt_cache_attend(const drt_cache_attend_args* args, void* stream);
+/* Scores of given tokens under softmax(x / T) (T <= 0: no scaling) of rows of logits (DRT_TYPE_*, row r or
+ * row_index[r], row stride ld): logprob[r] of tokens[r] (-inf for a token outside the vocabulary, whose rank
+ * is -1), entropy[r] in nats, rank[r] = tokens before it by (logit, lowest id), and the `top` (at most 32)
+ * likeliest tokens with their log probabilities in that order, -1 and -inf behind the last of non-zero
+ * probability. exclude_token (-1: none) counts as -inf. A row without any finite or +inf logit gives -inf,
+ * entropy 0 and no alternatives; a NaN in a row gives NaN log probabilities and entropy. Null outputs are
+ * left out. The selectors above score the argmax; this scores what was answered. */
+size_t drt_selector_logprobs_scratch_bytes(int32_t rows, int32_t vocab, int32_t dtype);
+int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, const int32_t* row_index, int32_t rows,
+                          int32_t vocab, const int32_t* tokens, double temperature, int32_t exclude_token, int32_t top,
+                          void* scratch, float* logprob, float* entropy, int32_t* rank, int32_t* top_token,
+                          float* top_logprob, void* stream);
 /* y = x @ W^T on the tensor cores with the MLX rounding contract (bf16 output rounding when
  * round_bf16 != 0). x [rows x K] bf16, w [n x K] bf16, y [rows x n] f32; n % 128 == 0,
  * K % 64 == 0; splits in {1, 2, 4, 8, 16} (split-K CTAs of a tile form one thread-block cluster
