@@ -47,10 +47,10 @@ struct CacheAttnArgs {
   int64_t out_row, out_head;
   float* lse;                 // [q_rows][heads * group] or null
   int vec;                    // q rows start on 16-byte boundaries
-  // partial sums of units cut between shares
-  float* part;                // [workers][2][rows of a tile][dim]
-  float4* stat;               // [workers][2][rows of a tile]: m, M, l
-  int4* desc;                 // [workers][2]
+  // parts of cut units: per warp and per CTA a front and a tail, [rows of a tile][dim] sums and their (m, M, l)
+  float *part, *cta_part;
+  float4 *stat, *cta_stat;
+  int4* desc;                 // [CTAs] rows | last CTA << 8, request, row tile, head of the unit that the CTA begins
 };
 
 struct CacheReq {
@@ -102,10 +102,18 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 }
 
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+
+// Transposed 8 x 8 matrix of f16 spread over the warp (a lane holds row lane / 4, columns 2 (lane % 4), + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t f16_pair(float x, float y) {
@@ -121,53 +129,82 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // ---------------------------------------------------------------- few rows: one warp, one share
-// A warp owns a share: row tiles of 16 (row = position * group + query head, so a kv head's keys serve all
-// of its query heads), mma.sync m16n8k16 with the codes read from its own ring of key and value tiles in
-// shared memory. With 16 rows the tiles are bound by their bytes (256 B per key and head against 8 kFLOP),
-// and the legacy matrix instruction needs no staging of expanded tiles: the codes become f16 operands in
-// the registers of the lane that read them. tcgen05 would need them expanded in shared memory first.
+// A warp owns a share. Its unit is a row tile of 8 kNT rows (row = position * group + query head, so a kv head's
+// keys serve all of its query heads) and it computes the transposed products on mma.sync m16n8k16,
+//   S^T [keys x rows] = K Q^T,   O^T [dims x rows] += V^T W^T,
+// with the codes as the 16-row operand: eight rows, the query heads of one token in a GQA model, then waste
+// nothing, and each code is expanded to f16 once, in the registers of the lane that read it. With so few rows the
+// tiles are bound by their bytes (256 B per key and head against 512 kNT MACs a byte pair needs); tcgen05 would
+// need the expanded codes written to shared memory first.
 //
-// Lanes (g = lane / 4, q = lane % 4). The contracted dimension may be taken in any order that both operands
-// share, so a lane's 16-byte read of a key's row is four k-steps' worth of its B fragment, and key n of score
-// tile j is token 16 (n / 2) + 2 j + n % 2 of the 64: then the score columns that a lane holds (2q, 2q + 1 of
-// each j) are tokens 16 q .. 16 q + 15, one 16-token group of V, whose codes are again one 16-byte read per
-// dimension, and one block (a block holds whole groups), so a lane needs one ks and one vs per tile.
+// Lanes (g = lane / 4, q = lane % 4). The contracted index may be taken in any order that both operands share:
+//   K: a lane reads 16 bytes of a key's row, dimensions 16 (q + 4 half) .., four k-steps' worth of its fragment;
+//   V: a lane reads the 16 tokens of group q of one dimension, four k-steps' worth; so k-step s of the 64 keys
+//      contracts tokens 16 q + 4 s + {0, 1} and + {2, 3} of each lane group q, and K's fragment s holds the same
+//      tokens in its rows: row g token 16 (g / 2) + 4 s + g % 2, row g + 8 the token two behind.
+// A lane's keys are all of group g / 2, hence of one block (a block holds whole groups): one ks, one vs per
+// lane and tile. movmatrix turns W^T's accumulator layout into the operand's.
 //
-// The warps do not wait for one another: each issues its own copies (2 KB per group), three tiles of K or V
-// ahead, and 8 warps keep about 130 KB of copies in flight per SM.
-constexpr int kQrWarps = 8;
-constexpr int kQrThreads = kQrWarps * 32;
-constexpr int kQrRows = 16;
+// The warps do not wait for one another until their shares are done: each issues its own copies (2 KB per 16-token
+// group) into its own ring of K and V tiles, on into its next unit, whose table entries it has read by then. At the
+// end the CTA joins what its warps' borders cut, so that a long unit leaves one part per CTA and not one per warp.
 constexpr int kQrTile = 64;        // keys
 constexpr int kQrMaxRequests = 16384;
 
-template <int kDim>
+template <int kDim, int kNT>
 struct QrCfg {
+  static constexpr int kRows = 8 * kNT;
+  static constexpr int kWarps = kNT == 1 ? 8 : 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kGroupBytes = 16 * kDim;
   static constexpr int kGroupPitch = kGroupBytes + 32;  // V reads of the four groups fall into different banks
   static constexpr int kSlot = 4 * kGroupPitch;
-  static constexpr int kSlots = kDim == 128 ? 3 : 6;
+  static constexpr int kSlots = (kWarps <= 8 ? 3 : 2) * (128 / kDim);
   static constexpr int kRing = kSlots * kSlot;
-  static constexpr size_t kSmem = static_cast<size_t>(kQrWarps) * kRing + kQrWarps * kSlots * 8;
+  static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kRing + kWarps * kSlots * 8;
+};
+constexpr int kQrMaxRows = 16;                 // of a tile
+constexpr int kQrMaxParts = 8 * 2 * kQrMaxRows;  // rows of the parts of a CTA's warps
+
+// A unit: row tile t of request r with kv head h. lim: the keys that its last row sees, L: their tiles (at least one).
+struct QaUnit {
+  CacheReq q;
+  int r, t, h, lim, L;
 };
 
-// Key tiles of row tile t.
 template <int kRows, int kTile>
-__device__ __forceinline__ int qa_tiles(const CacheAttnArgs& a, const CacheReq& q, int t) {
-  const int last = min(q.n * a.group, (t + 1) * kRows) - 1;
-  return max(1, (cache_limit(a, q, last / a.group) + kTile - 1) / kTile);
+__device__ __forceinline__ void qa_size(const CacheAttnArgs& a, QaUnit& u) {
+  u.lim = cache_limit(a, u.q, (min(u.q.n * a.group, (u.t + 1) * kRows) - 1) / a.group);
+  u.L = max(1, (u.lim + kTile - 1) / kTile);
+}
+// The unit behind u; there is one.
+template <int kRows, int kTile>
+__device__ __forceinline__ void qa_next(const CacheAttnArgs& a, QaUnit& u) {
+  if (++u.h < a.heads) return;
+  u.h = 0;
+  if (++u.t * kRows >= u.q.n * a.group) {
+    u.t = 0;
+    do u.q = cache_request(a, ++u.r);
+    while (u.q.n == 0);
+  }
+  qa_size<kRows, kTile>(a, u);
 }
 
-__device__ __forceinline__ int64_t qa_share(int64_t total, int workers, int w) { return total * w / workers; }
+__device__ __forceinline__ int64_t qa_share(int64_t total, int shares, int w) { return total * w / shares; }
 // The share that holds tile x.
-__device__ __forceinline__ int qa_owner(int64_t total, int workers, int64_t x) {
-  int w = static_cast<int>(x * workers / total);
-  while (w + 1 < workers && qa_share(total, workers, w + 1) <= x) ++w;
-  while (w > 0 && qa_share(total, workers, w) > x) --w;
+__device__ __forceinline__ int qa_owner(int64_t total, int shares, int64_t x) {
+  int w = static_cast<int>(x * shares / total);
+  while (w + 1 < shares && qa_share(total, shares, w + 1) <= x) ++w;
+  while (w > 0 && qa_share(total, shares, w) > x) --w;
   return w;
 }
 
-// Exclusive sums of the requests' tile counts into prefix[0 .. requests], by the whole CTA.
+// What a unit costs beside its tiles, in tiles: the reads of its queries and table, its softmax's start and its output.
+// A unit takes so many places on the axis before its first tile, so that the shares of many short units are not
+// longer than those of one long one.
+constexpr int kQaUnitCost = 2;
+
+// Exclusive sums of the requests' places on the axis into prefix[0 .. requests], by the whole CTA.
 template <int kRows, int kTile, int kThreads>
 __device__ __forceinline__ int64_t qa_prefix(const CacheAttnArgs& a, int64_t* prefix) {
   __shared__ int64_t wsum[kThreads / 32];
@@ -179,7 +216,12 @@ __device__ __forceinline__ int64_t qa_prefix(const CacheAttnArgs& a, int64_t* pr
     if (r < a.requests) {
       const CacheReq q = cache_request(a, r);
       const int nt = (q.n * a.group + kRows - 1) / kRows;
-      for (int t = 0; t < nt; ++t) v += qa_tiles<kRows, kTile>(a, q, t);
+      QaUnit u;
+      u.q = q;
+      for (u.t = 0; u.t < nt; ++u.t) {
+        qa_size<kRows, kTile>(a, u);
+        v += u.L + kQaUnitCost;
+      }
       v *= a.heads;
     }
     int64_t x = v;
@@ -216,13 +258,48 @@ __device__ __forceinline__ void qa_store2<__nv_bfloat16>(__nv_bfloat16* p, float
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
 }
 
-template <typename T, int kDim, int kCode>
-__global__ void __launch_bounds__(kQrThreads, 1) cache_attn_rows_kernel(const CacheAttnArgs a) {
-  using Cfg = QrCfg<kDim>;
+// What a warp's share cuts: its front (a unit begun in an earlier share) and its tail (one that ends in a later).
+enum : int { QR_FRONT = 1, QR_FRONT_ENDS = 2, QR_TAIL = 4 };
+struct QrEnd {
+  int flags, rows, front_rows, busy, r, t, h, last;
+};
+
+template <int kE>
+__device__ __forceinline__ void qa_load(float* v, const float* src) {
+  if constexpr (kE == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(src);
+    v[0] = x.x;
+    v[1] = x.y;
+    v[2] = x.z;
+    v[3] = x.w;
+  } else {
+    const float2 x = *reinterpret_cast<const float2*>(src);
+    v[0] = x.x;
+    v[1] = x.y;
+  }
+}
+
+// A finished row by one warp: kE dimensions a lane, sums against the references z (of l) and Z (of acc).
+template <typename T, int kE>
+__device__ __forceinline__ void qa_put(const CacheAttnArgs& a, int r, int row, int h, int lane, float z, float Z, float m,
+                                       float l, const float* acc) {
+  const int i = row / a.group, hq = h * a.group + row - i * a.group;
+  const int64_t out_row = min(max(a.row_start[r], 0), a.q_rows) + i;
+  const float n = l == 0.0f ? 0.0f : qa_ex2(Z - z) / l;
+  T* dst = static_cast<T*>(a.out) + out_row * a.out_row + hq * a.out_head + lane * kE;
+#pragma unroll
+  for (int e = 0; e < kE; e += 2) qa_store2<T>(dst + e, acc[e] * n, acc[e + 1] * n);
+  if (lane == 0 && a.lse) a.lse[out_row * a.heads * a.group + hq] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <typename T, int kDim, int kCode, int kNT>
+__global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows_kernel(const CacheAttnArgs a) {
+  using Cfg = QrCfg<kDim, kNT>;
+  constexpr int kRows = Cfg::kRows;
   constexpr int kHalves = kDim / 64;   // 16-byte reads of a key's row per lane
-  constexpr int kDTiles = kDim / 8;
+  constexpr int kMT = kDim / 16;       // 16-dimension tiles of O^T
   extern __shared__ __align__(128) uint8_t qr_smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qr_smem + kQrWarps * Cfg::kRing);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(qr_smem + Cfg::kWarps * Cfg::kRing);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, tq = lane & 3;
   uint8_t* ring = qr_smem + warp * Cfg::kRing;
@@ -231,434 +308,551 @@ __global__ void __launch_bounds__(kQrThreads, 1) cache_attn_rows_kernel(const Ca
     for (int i = 0; i < Cfg::kSlots; ++i) mbar_init(&full[i], 1);
   fence_mbar_init();
 
+  __shared__ QrEnd ends[Cfg::kWarps];
   int64_t* prefix = reinterpret_cast<int64_t*>(qr_smem);
-  const int64_t total = qa_prefix<kQrRows, kQrTile, kQrThreads>(a, prefix);
-  const int workers = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x) * kQrWarps));
-  const int me = warp * gridDim.x + blockIdx.x;   // few tiles spread over the CTAs first
+  const int64_t total = qa_prefix<kRows, kQrTile, Cfg::kThreads>(a, prefix);
+  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
   int64_t x = 0, x_end = 0;
-  int r = 0;
-  if (me < workers) {
-    x = qa_share(total, workers, me);
-    x_end = qa_share(total, workers, me + 1);
+  QaUnit cur = {};
+  if (blockIdx.x < ctas) {
+    const int64_t c0 = qa_share(total, ctas, blockIdx.x), n = qa_share(total, ctas, blockIdx.x + 1) - c0;
+    x = c0 + qa_share(n, Cfg::kWarps, warp);
+    x_end = c0 + qa_share(n, Cfg::kWarps, warp + 1);
     int hi = a.requests;
-    while (hi - r > 1) {
-      const int mid = (r + hi) >> 1;
-      if (prefix[mid] <= x) r = mid;
+    while (hi - cur.r > 1) {
+      const int mid = (cur.r + hi) >> 1;
+      if (prefix[mid] <= x) cur.r = mid;
       else hi = mid;
     }
   }
-  const int64_t r_first = prefix[r];
+  int64_t rem = x - prefix[cur.r];
   __syncthreads();           // prefix is done with: its memory becomes the rings
   fence_proxy_async_smem();
-  if (me >= workers) {
-    if (lane == 0) a.desc[me * 2] = make_int4(0, 0, 0, 0);
-    return;
-  }
 
-  CacheReq rq = cache_request(a, r);
-  int t = 0, L = qa_tiles<kQrRows, kQrTile>(a, rq, 0);
-  int64_t rem = x - r_first;
-  while (rem >= static_cast<int64_t>(L) * a.heads) {
-    rem -= static_cast<int64_t>(L) * a.heads;
-    L = qa_tiles<kQrRows, kQrTile>(a, rq, ++t);
-  }
-  int h = static_cast<int>(rem / L), kt = static_cast<int>(rem % L);
-  uint32_t seq_used = 0;     // ring entries consumed so far
-  int4 owner = make_int4(0, 0, 0, 0), owner2 = owner;
-  uint32_t issued = 0;       // ring entries asked for so far
+  int kt = 0;                // first key tile of the segment: what this share holds of the unit
+  uint32_t seq_used = 0;     // ring entries consumed in earlier segments
+  uint32_t issued = 0;       // entries asked for, counted from the segment's first
   bool failed = false;
+  const int block_shift = 31 - __clz(a.block);
+  if (x < x_end) {
+    cur.q = cache_request(a, cur.r);
+    qa_size<kRows, kQrTile>(a, cur);
+    while (rem >= static_cast<int64_t>(cur.L + kQaUnitCost) * a.heads) {
+      rem -= static_cast<int64_t>(cur.L + kQaUnitCost) * a.heads;
+      ++cur.t;
+      qa_size<kRows, kQrTile>(a, cur);
+    }
+    cur.h = static_cast<int>(rem / (cur.L + kQaUnitCost));
+    kt = static_cast<int>(rem % (cur.L + kQaUnitCost)) - kQaUnitCost;
+    if (kt < 0) {            // the share begins before the unit's first tile
+      x -= kt;
+      kt = 0;
+    }
+  }
+  QrEnd end;
+  end.flags = end.rows = end.front_rows = end.r = end.t = end.h = end.last = 0;
+  end.busy = x < x_end;
+  // tables and scales of eight tiles at a time: lane = tile * 4 + group
+  struct Meta {
+    int page;
+    float ks, vs;
+  };
+  auto table_entry = [&](const QaUnit& u, int tile0) {
+    const int tok = (tile0 + (lane >> 2)) * kQrTile + (lane & 3) * 16;
+    return tok < u.lim ? a.tables[u.r * a.ld_tables + (tok >> block_shift)] : -1;
+  };
+  auto scales_of = [&](int id, int h) {
+    Meta d = {-1, 0.0f, 0.0f};
+    if (id >= 0 && id < a.blocks) {
+      d.page = id;
+      d.ks = a.k_scale[static_cast<int64_t>(id) * a.heads + h];
+      d.vs = a.v_scale[static_cast<int64_t>(id) * a.heads + h];
+    }
+    return d;
+  };
+  int tiles = static_cast<int>(min(static_cast<int64_t>(cur.L - kt), x_end - x));
+  QaUnit nxt = cur;
+  Meta now = {-1, 0.0f, 0.0f}, then = now, ahead = now;
+  if (x < x_end) now = scales_of(table_entry(cur, kt), cur.h);
 
   while (x < x_end && !failed) {
-    const int tiles = static_cast<int>(min(static_cast<int64_t>(L - kt), x_end - x));
-    const int rows_all = rq.n * a.group;
-    const int row_a = t * kQrRows + g, row_b = row_a + 8;
-    const bool ok_a = row_a < rows_all, ok_b = row_b < rows_all;
-    const int i_a = min(row_a, rows_all - 1) / a.group, i_b = min(row_b, rows_all - 1) / a.group;
-    const int lim_a = cache_limit(a, rq, i_a), lim_b = cache_limit(a, rq, i_b);
-    const int lim = cache_limit(a, rq, (min(rows_all, (t + 1) * kQrRows) - 1) / a.group);  // the tile's largest
-    const int hq_a = h * a.group + min(row_a, rows_all - 1) - i_a * a.group;
-    const int hq_b = h * a.group + min(row_b, rows_all - 1) - i_b * a.group;
-
-    // ---- tables and scales of eight tiles at a time: lane = tile * 4 + group
-    int page, page_n;
-    float ks, lv, ks_n, lv_n;
-    const int* table = a.tables + r * a.ld_tables;
-    auto load_meta = [&](int tile0, int& pg, float& k, float& l) {
-      const int tok = (tile0 + (lane >> 2)) * kQrTile + (lane & 3) * 16;
-      pg = -1;
-      k = 0.0f;
-      l = -INFINITY;
-      if (tok < lim) {
-        const int id = table[tok / a.block];
-        if (id >= 0 && id < a.blocks) {
-          pg = id;
-          k = a.k_scale[static_cast<int64_t>(id) * a.heads + h] * a.scale_log2;
-          l = log2f(a.v_scale[static_cast<int64_t>(id) * a.heads + h]);
-        }
+    const int entries = 2 * tiles;
+    const int tiles_nxt = [&] {
+      if (x + tiles + kQaUnitCost >= x_end) return 0;
+      qa_next<kRows, kQrTile>(a, nxt);
+      return static_cast<int>(min(static_cast<int64_t>(nxt.L), x_end - x - tiles - kQaUnitCost));
+    }();
+    // Asks for the next ring entry (even: K, odd: V) of this segment or the one behind it; `done` tiles are consumed.
+    auto issue = [&](int done) -> bool {
+      int s = issued, base = kt, h = cur.h, pg;
+      if (s < entries) {
+        const int tile = s >> 1;
+        pg = __shfl_sync(~0u, (tile >> 3) != (done >> 3) ? then.page : now.page, (tile & 7) * 4 + (lane & 3));
+      } else {
+        s -= entries;
+        if (s >= 2 * tiles_nxt || s >= 16) return false;
+        base = 0;
+        h = nxt.h;
+        pg = __shfl_sync(~0u, ahead.page, (s >> 1) * 4 + (lane & 3));
       }
-    };
-    load_meta(kt, page, ks, lv);
-    load_meta(kt + 8, page_n, ks_n, lv_n);
-
-    auto issue = [&](int s, int done) {  // ring entry s of this segment (even: K, odd: V); `done` tiles consumed
-      const int tile = s >> 1;
-      const bool next = (tile >> 3) != (done >> 3);
-      const int pg = __shfl_sync(~0u, next ? page_n : page, (tile & 7) * 4 + (lane & 3));
-      const uint32_t e = seq_used + s;
-      const int slot = e % Cfg::kSlots;
-      issued = e + 1;
+      const uint32_t slot = (seq_used + issued++) % Cfg::kSlots;
       const uint32_t have = __ballot_sync(~0u, pg >= 0) & 15u;
       if (lane == 0) mbar_expect_tx(&full[slot], __popc(have) * Cfg::kGroupBytes);
       __syncwarp();
       if (lane < 4 && pg >= 0) {
-        const int tok = (kt + tile) * kQrTile + lane * 16;
+        const int tok = (base + (s >> 1)) * kQrTile + lane * 16;
         const uint8_t* src = ((s & 1) ? a.v_cache : a.k_cache) +
-                             ((static_cast<int64_t>(pg) * a.heads + h) * a.block + tok % a.block) * kDim;
+                             (((static_cast<int64_t>(pg) * a.heads + h) << block_shift) + (tok & (a.block - 1))) * kDim;
         bulk_load(smem_u32(ring + slot * Cfg::kSlot + lane * Cfg::kGroupPitch), src, Cfg::kGroupBytes, &full[slot]);
       }
+      return true;
     };
-    const int entries = 2 * tiles;
-    for (int s = 0; s < min(Cfg::kSlots, entries); ++s) issue(s, 0);
-
-    // ---- Q fragments: lane holds dimensions 16 (q + 4 half) .. + 15 of rows g and g + 8
-    uint32_t qf[kHalves * 4][4];
-    float f_a = 1.0f, f_b = 1.0f;  // takes a bf16 row's power of two back
-    {
-      const T* qa = static_cast<const T*>(a.q) + (rq.row0 + i_a) * a.q_row + hq_a * a.q_head;
-      const T* qb = static_cast<const T*>(a.q) + (rq.row0 + i_b) * a.q_row + hq_b * a.q_head;
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const T* src = side ? qb : qa;
-        __align__(16) T v[kHalves * 16];
-#pragma unroll
-        for (int hh = 0; hh < kHalves; ++hh) {
-          const T* p = src + 16 * (tq + 4 * hh);
-          if (a.vec) {
-            reinterpret_cast<uint4*>(v)[hh * 2] = reinterpret_cast<const uint4*>(p)[0];
-            reinterpret_cast<uint4*>(v)[hh * 2 + 1] = reinterpret_cast<const uint4*>(p)[1];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[hh * 16 + i] = p[i];
-          }
-        }
-        float up = 1.0f;
-        if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-          float mx = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kHalves * 16; ++i) mx = fmaxf(mx, fabsf(cache_in_f32(v[i])));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-          // the largest magnitude to [2^14, 2^15)
-          const int e = mx > 0.0f && mx <= 3.402823466e38f ? max(-100, static_cast<int>((__float_as_uint(mx) >> 23) & 255) - 127) : 14;
-          up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-          const float down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
-          if (side) f_b = down;
-          else f_a = down;
-        }
-#pragma unroll
-        for (int st = 0; st < kHalves * 4; ++st) {
-          qf[st][side] = f16_pair(cache_in_f32(v[st * 4]) * up, cache_in_f32(v[st * 4 + 1]) * up);
-          qf[st][2 + side] = f16_pair(cache_in_f32(v[st * 4 + 2]) * up, cache_in_f32(v[st * 4 + 3]) * up);
-        }
-      }
+    while (issued < Cfg::kSlots && issued < entries) issue(0);
+    // asked for here, looked at behind the first K tile's products
+    int then_id = tiles > 8 ? table_entry(cur, kt + 8) : -1;
+    const int ahead_id = tiles_nxt > 0 ? table_entry(nxt, 0) : -1;
+    const int rows_all = cur.q.n * a.group, row0 = cur.t * kRows, lim = cur.lim;
+    if (tiles_nxt > 0) {     // the next unit's rows of Q on their way to L2
+      const int row = min(nxt.t * kRows + g, nxt.q.n * a.group - 1), i = row / a.group;
+      const T* src = static_cast<const T*>(a.q) + (nxt.q.row0 + i) * a.q_row + (nxt.h * a.group + row - i * a.group) * a.q_head;
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(src + tq * (kDim / 4)));
     }
 
-    float o[kDTiles][4];
+    // ---- Q^T fragments: lane holds dimensions 16 (q + 4 half) .. + 15 of row g of each row group
+    uint32_t qf[kNT][kHalves * 4][2];
+    float f[kNT];             // takes the power of two of row g back
 #pragma unroll
-    for (int i = 0; i < kDTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m_a = -INFINITY, m_b = -INFINITY, M_a = -INFINITY, M_b = -INFINITY, l_a = 0.0f, l_b = 0.0f;
+    for (int n = 0; n < kNT; ++n) {
+      const int row = min(row0 + n * 8 + g, rows_all - 1), i = row / a.group;
+      const T* src = static_cast<const T*>(a.q) + (cur.q.row0 + i) * a.q_row + (cur.h * a.group + row - i * a.group) * a.q_head;
+      __align__(16) T v[kHalves * 16];
+#pragma unroll
+      for (int hh = 0; hh < kHalves; ++hh) {
+        const T* p = src + 16 * (tq + 4 * hh);
+        if (a.vec) {
+          reinterpret_cast<uint4*>(v)[hh * 2] = reinterpret_cast<const uint4*>(p)[0];
+          reinterpret_cast<uint4*>(v)[hh * 2 + 1] = reinterpret_cast<const uint4*>(p)[1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[hh * 16 + e] = p[e];
+        }
+      }
+      float up = 1.0f;
+      f[n] = a.scale_log2;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kHalves * 16; ++e) mx = fmaxf(mx, fabsf(cache_in_f32(v[e])));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        // the largest magnitude to [2^14, 2^15)
+        const int e = mx > 0.0f && mx <= 3.402823466e38f ? max(-100, static_cast<int>((__float_as_uint(mx) >> 23) & 255) - 127) : 14;
+        up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+        f[n] *= __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+      }
+#pragma unroll
+      for (int st = 0; st < kHalves * 4; ++st) {
+        qf[n][st][0] = f16_pair(cache_in_f32(v[st * 4]) * up, cache_in_f32(v[st * 4 + 1]) * up);
+        qf[n][st][1] = f16_pair(cache_in_f32(v[st * 4 + 2]) * up, cache_in_f32(v[st * 4 + 3]) * up);
+      }
+    }
+    // of the rows that this lane's accumulators hold: 2 q and 2 q + 1 of each row group
+    float fr[kNT][2];
+    int lr[kNT][2], lim_low = lim;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        fr[n][e] = __shfl_sync(~0u, f[n], (2 * tq + e) * 4);
+        lr[n][e] = cache_limit(a, cur.q, min(row0 + n * 8 + 2 * tq + e, rows_all - 1) / a.group);
+        lim_low = min(lim_low, lr[n][e]);
+      }
+
+    float o[kNT][kMT][4];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+    float m[kNT][2], M[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = M[n][e] = -INFINITY;
+        l[n][e] = 0.0f;
+      }
 
     for (int j = 0; j < tiles; ++j) {
       if (j > 0 && (j & 7) == 0) {
-        page = page_n;
-        ks = ks_n;
-        lv = lv_n;
-        load_meta(kt + j + 8, page_n, ks_n, lv_n);
+        now = then;
+        then_id = j + 8 < tiles ? table_entry(cur, kt + j + 8) : -1;
       }
-      const int src_lane = (j & 7) * 4 + tq;
-      const float k_mul = __shfl_sync(~0u, ks, src_lane), lv_g = __shfl_sync(~0u, lv, src_lane);
-      const bool here = __shfl_sync(~0u, page, src_lane) >= 0;
       const int key0 = (kt + j) * kQrTile;
 
-      // ---- S = Q K^T
-      float s[8][4];
+      // ---- S^T = K Q^T
+      float s[kNT][4][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.0f;
       {
         const uint32_t e = seq_used + 2 * j;
         if (!failed) failed = __any_sync(~0u, !mbar_wait(&full[e % Cfg::kSlots], (e / Cfg::kSlots) & 1));
         const uint8_t* kb = ring + (e % Cfg::kSlots) * Cfg::kSlot + (g >> 1) * Cfg::kGroupPitch + (g & 1) * kDim + tq * 16;
+        // four keys' fragments side by side: their products do not wait for one another
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int hh = 0; hh < kHalves; ++hh) {
+          uint4 u[4], u2[4];
 #pragma unroll
-          for (int hh = 0; hh < kHalves; ++hh) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kb + 2 * i * kDim + hh * 64);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-              uint32_t b0, b1;
-              codes_to_f16<kCode>(w[st], b0, b1);
-              mma_f16(s[i], qf[hh * 4 + st], b0, b1);
-            }
+          for (int i = 0; i < 4; ++i) {
+            u[i] = *reinterpret_cast<const uint4*>(kb + 4 * i * kDim + hh * 64);
+            u2[i] = *reinterpret_cast<const uint4*>(kb + (4 * i + 2) * kDim + hh * 64);
           }
+#pragma unroll
+          for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t af[4];
+              codes_to_f16<kCode>(word_of(u[i], st), af[0], af[2]);
+              codes_to_f16<kCode>(word_of(u2[i], st), af[1], af[3]);
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) mma_f16(s[n][i], af, qf[n][hh * 4 + st][0], qf[n][hh * 4 + st][1]);
+            }
         }
         __syncwarp();
-        if (!failed && 2 * j + Cfg::kSlots < entries) issue(2 * j + Cfg::kSlots, j);
+        if ((j & 7) == 0) then = scales_of(then_id, cur.h);
+        if (j == 0) ahead = scales_of(ahead_id, nxt.h);
+        while (!failed && issued < 2 * j + 1 + Cfg::kSlots && issue(j)) {}
       }
 
-      // ---- softmax
-      const float c_a = k_mul * f_a, c_b = k_mul * f_b;
-      const int first = key0 + tq * 16;
-      if (__any_sync(~0u, key0 + kQrTile > min(lim_a, lim_b) || !here)) {
+      // ---- softmax over this lane's eight keys, then over the lanes g of a row
+      const int src_lane = (j & 7) * 4 + (g >> 1);
+      const float k_mul = __shfl_sync(~0u, now.ks, src_lane), lv = __log2f(__shfl_sync(~0u, now.vs, src_lane));
+      const bool here = __shfl_sync(~0u, now.page, src_lane) >= 0;
+      const int first = key0 + (g >> 1) * 16 + (g & 1);  // the lane's keys: first + 4 i, + 2
+      const bool edge = __any_sync(~0u, key0 + kQrTile > lim_low || !here);
+      uint32_t pf[kNT][4][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+      for (int n = 0; n < kNT; ++n) {
+        float tm[2], um[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float c = k_mul * fr[n][e];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[n][i][e] *= c;
+            s[n][i][2 + e] *= c;
+          }
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (!(here && first + 4 * i < lr[n][e])) s[n][i][e] = -INFINITY;
+              if (!(here && first + 4 * i + 2 < lr[n][e])) s[n][i][2 + e] = -INFINITY;
+            }
+          }
+          tm[e] = fmaxf(s[n][0][e], s[n][0][2 + e]);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) tm[e] = fmaxf(tm[e], fmaxf(s[n][i][e], s[n][i][2 + e]));
+          um[e] = here ? tm[e] + lv : -INFINITY;
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            s[i][e] = here && first + 2 * i + e < lim_a ? s[i][e] * c_a : -INFINITY;
-            s[i][2 + e] = here && first + 2 * i + e < lim_b ? s[i][2 + e] * c_b : -INFINITY;
+            tm[e] = fmaxf(tm[e], __shfl_xor_sync(~0u, tm[e], d));
+            um[e] = fmaxf(um[e], __shfl_xor_sync(~0u, um[e], d));
+          }
+        float z[2], w[2], k[2];
+        bool moved = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float nm = fmaxf(m[n][e], tm[e]), nM = fmaxf(M[n][e], um[e]);
+          // a row that has seen nothing yet keeps zeros: its reference is 0 and every term 2^-inf
+          z[e] = nm == -INFINITY ? 0.0f : nm;
+          const float Z = nM == -INFINITY ? 0.0f : nM;
+          l[n][e] *= qa_ex2(m[n][e] - z[e]);
+          k[e] = qa_ex2(M[n][e] - Z);
+          moved = moved || nM != M[n][e];
+          m[n][e] = nm;
+          M[n][e] = nM;
+          // weight = p vs / 2^(M - m): at most 1 where p is not 0; the factor alone may leave f32's range
+          w[e] = here ? qa_ex2(fminf(lv + (z[e] - Z), 120.0f)) : 0.0f;
+        }
+        if (__any_sync(~0u, moved)) {
+#pragma unroll
+          for (int i = 0; i < kMT; ++i) {
+            o[n][i][0] *= k[0];
+            o[n][i][1] *= k[1];
+            o[n][i][2] *= k[0];
+            o[n][i][3] *= k[1];
           }
         }
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          s[i][0] *= c_a;
-          s[i][1] *= c_a;
-          s[i][2] *= c_b;
-          s[i][3] *= c_b;
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = qa_ex2(s[n][i][0] - z[0]), p1 = qa_ex2(s[n][i][1] - z[1]);
+          const float p2 = qa_ex2(s[n][i][2] - z[0]), p3 = qa_ex2(s[n][i][3] - z[1]);
+          l[n][0] += p0 + p2;
+          l[n][1] += p1 + p3;
+          pf[n][i][0] = transpose8(f16_pair(p0 * w[0], p1 * w[1]));
+          pf[n][i][1] = transpose8(f16_pair(p2 * w[0], p3 * w[1]));
         }
-      }
-      float t_a = s[0][0], t_b = s[0][2];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        t_a = fmaxf(t_a, fmaxf(s[i][0], s[i][1]));
-        t_b = fmaxf(t_b, fmaxf(s[i][2], s[i][3]));
-      }
-      float u_a = t_a + lv_g, u_b = t_b + lv_g;
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        t_a = fmaxf(t_a, __shfl_xor_sync(~0u, t_a, d));
-        t_b = fmaxf(t_b, __shfl_xor_sync(~0u, t_b, d));
-        u_a = fmaxf(u_a, __shfl_xor_sync(~0u, u_a, d));
-        u_b = fmaxf(u_b, __shfl_xor_sync(~0u, u_b, d));
-      }
-      const float nm_a = fmaxf(m_a, t_a), nm_b = fmaxf(m_b, t_b);
-      const float nM_a = fmaxf(M_a, u_a), nM_b = fmaxf(M_b, u_b);
-      // a row that has seen nothing yet keeps zeros: its reference is 0 and every term 2^-inf
-      const float z_a = nm_a == -INFINITY ? 0.0f : nm_a, z_b = nm_b == -INFINITY ? 0.0f : nm_b;
-      const float Z_a = nM_a == -INFINITY ? 0.0f : nM_a, Z_b = nM_b == -INFINITY ? 0.0f : nM_b;
-      l_a *= qa_ex2(m_a - z_a);
-      l_b *= qa_ex2(m_b - z_b);
-      if (__any_sync(~0u, nM_a != M_a || nM_b != M_b)) {
-        const float k_a = qa_ex2(M_a - Z_a), k_b = qa_ex2(M_b - Z_b);
-#pragma unroll
-        for (int i = 0; i < kDTiles; ++i) {
-          o[i][0] *= k_a;
-          o[i][1] *= k_a;
-          o[i][2] *= k_b;
-          o[i][3] *= k_b;
-        }
-      }
-      m_a = nm_a;
-      m_b = nm_b;
-      M_a = nM_a;
-      M_b = nM_b;
-      // w = p vs / 2^(M - m): at most 1 where p is not 0; the factor alone may leave f32's range
-      const float w_a = qa_ex2(fminf(lv_g + (z_a - Z_a), 120.0f)), w_b = qa_ex2(fminf(lv_g + (z_b - Z_b), 120.0f));
-      uint32_t pf[4][4];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p0 = qa_ex2(s[i][0] - z_a), p1 = qa_ex2(s[i][1] - z_a);
-        const float p2 = qa_ex2(s[i][2] - z_b), p3 = qa_ex2(s[i][3] - z_b);
-        l_a += p0 + p1;
-        l_b += p2 + p3;
-        pf[i >> 1][(i & 1) * 2] = f16_pair(p0 * w_a, p1 * w_a);
-        pf[i >> 1][(i & 1) * 2 + 1] = f16_pair(p2 * w_b, p3 * w_b);
       }
 
-      // ---- O += W V
+      // ---- O^T += V^T W^T
       {
         const uint32_t e = seq_used + 2 * j + 1;
         if (!failed) failed = __any_sync(~0u, !mbar_wait(&full[e % Cfg::kSlots], (e / Cfg::kSlots) & 1));
         const uint8_t* vb = ring + (e % Cfg::kSlots) * Cfg::kSlot + tq * Cfg::kGroupPitch + g * 16;
         // tokens nobody sees hold anything: their codes are cleared, since 0 times a NaN code is not 0
-        const int live = here ? min(16, max(0, lim - first)) : 0;
-        uint32_t keep[4];
+        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+        if (edge) {
+          const bool mine = __shfl_sync(~0u, now.page, (j & 7) * 4 + tq) >= 0;
+          const int live = mine ? min(16, max(0, lim - key0 - tq * 16)) : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = min(4, max(0, live - 4 * i));
-          keep[i] = n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
-        }
-#pragma unroll
-        for (int i = 0; i < kDTiles; ++i) {
-          const uint4 u = *reinterpret_cast<const uint4*>(vb + i * 128);
-          const uint32_t w[4] = {u.x & keep[0], u.y & keep[1], u.z & keep[2], u.w & keep[3]};
-#pragma unroll
-          for (int st = 0; st < 4; ++st) {
-            uint32_t b0, b1;
-            codes_to_f16<kCode>(w[st], b0, b1);
-            mma_f16(o[i], pf[st], b0, b1);
+          for (int i = 0; i < 4; ++i) {
+            const int c = min(4, max(0, live - 4 * i));
+            keep[i] = c >= 4 ? ~0u : (1u << (8 * c)) - 1u;
           }
         }
+#pragma unroll
+        for (int i0 = 0; i0 < kMT; i0 += 4) {
+          uint4 u[4], u2[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            u[i] = *reinterpret_cast<const uint4*>(vb + (i0 + i) * 256);
+            u2[i] = *reinterpret_cast<const uint4*>(vb + (i0 + i) * 256 + 128);
+          }
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              u[i] = make_uint4(u[i].x & keep[0], u[i].y & keep[1], u[i].z & keep[2], u[i].w & keep[3]);
+              u2[i] = make_uint4(u2[i].x & keep[0], u2[i].y & keep[1], u2[i].z & keep[2], u2[i].w & keep[3]);
+            }
+          }
+#pragma unroll
+          for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t af[4];
+              codes_to_f16<kCode>(word_of(u[i], st), af[0], af[2]);
+              codes_to_f16<kCode>(word_of(u2[i], st), af[1], af[3]);
+#pragma unroll
+              for (int n = 0; n < kNT; ++n) mma_f16(o[n][i0 + i], af, pf[n][st][0], pf[n][st][1]);
+            }
+        }
         __syncwarp();
-        if (!failed && 2 * j + 1 + Cfg::kSlots < entries) issue(2 * j + 1 + Cfg::kSlots, j);
+        while (!failed && issued < 2 * j + 2 + Cfg::kSlots && issue(j)) {}
       }
     }
-    seq_used += entries;
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      l_a += __shfl_xor_sync(~0u, l_a, d);
-      l_b += __shfl_xor_sync(~0u, l_b, d);
-    }
-    if (failed) l_a = l_b = NAN;  // a copy did not arrive in time: the rows read as NaN
 
-    const bool begins = kt == 0, ends = kt + tiles == L;
-    if (begins && ends) {
-      T* out = static_cast<T*>(a.out);
-      const float n_a = l_a == 0.0f ? 0.0f : qa_ex2(M_a - m_a) / l_a, n_b = l_b == 0.0f ? 0.0f : qa_ex2(M_b - m_b) / l_b;
-      T* pa = out + (rq.row0 + i_a) * a.out_row + hq_a * a.out_head + 2 * tq;
-      T* pb = out + (rq.row0 + i_b) * a.out_row + hq_b * a.out_head + 2 * tq;
+    const bool begins = kt == 0, whole = begins && tiles == cur.L;
+    const int64_t at = (static_cast<int64_t>(blockIdx.x * Cfg::kWarps + warp) * 2 + (begins ? 1 : 0)) * kRows;
 #pragma unroll
-      for (int i = 0; i < kDTiles; ++i) {
-        if (ok_a) qa_store2<T>(pa + i * 8, o[i][0] * n_a, o[i][1] * n_a);
-        if (ok_b) qa_store2<T>(pb + i * 8, o[i][2] * n_b, o[i][3] * n_b);
-      }
-      if (a.lse && tq == 0) {
-        const int64_t hq = static_cast<int64_t>(a.heads) * a.group;
-        if (ok_a) a.lse[(rq.row0 + i_a) * hq + hq_a] = (m_a + log2f(l_a)) * 0.6931471805599453f;
-        if (ok_b) a.lse[(rq.row0 + i_b) * hq + hq_b] = (m_b + log2f(l_b)) * 0.6931471805599453f;
-      }
-    } else {
-      const int64_t at = (static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) * kQrRows;
-      float* pa = a.part + (at + g) * kDim + 2 * tq;
-      float* pb = pa + 8 * kDim;
+    for (int n = 0; n < kNT; ++n)
 #pragma unroll
-      for (int i = 0; i < kDTiles; ++i) {
-        if (ok_a) *reinterpret_cast<float2*>(pa + i * 8) = make_float2(o[i][0], o[i][1]);
-        if (ok_b) *reinterpret_cast<float2*>(pb + i * 8) = make_float2(o[i][2], o[i][3]);
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(~0u, l[n][e], d);
+        if (failed) l[n][e] = NAN;  // a copy did not arrive in time: the rows read as NaN
+        const int rt = n * 8 + 2 * tq + e, row = row0 + rt;
+        if (row >= rows_all) continue;
+        if (whole) {
+          const int i = row / a.group, hq = cur.h * a.group + row - i * a.group;
+          const float inv = l[n][e] == 0.0f ? 0.0f : qa_ex2(M[n][e] - m[n][e]) / l[n][e];
+          T* dst = static_cast<T*>(a.out) + (cur.q.row0 + i) * a.out_row + hq * a.out_head + g;
+#pragma unroll
+          for (int d = 0; d < kMT; ++d) {
+            dst[d * 16] = cache_out<T>(o[n][d][e] * inv);
+            dst[d * 16 + 8] = cache_out<T>(o[n][d][2 + e] * inv);
+          }
+          if (a.lse && g == 0)
+            a.lse[(cur.q.row0 + i) * static_cast<int64_t>(a.heads) * a.group + hq] =
+                (m[n][e] + log2f(l[n][e])) * 0.6931471805599453f;
+        } else {
+          float* dst = a.part + (at + rt) * kDim + g;
+#pragma unroll
+          for (int d = 0; d < kMT; ++d) {
+            dst[d * 16] = o[n][d][e];
+            dst[d * 16 + 8] = o[n][d][2 + e];
+          }
+          if (g == 0) a.stat[at + rt] = make_float4(m[n][e], M[n][e], l[n][e], 0.0f);
+        }
       }
-      if (tq == 0) {
-        if (ok_a) a.stat[at + g] = make_float4(m_a, M_a, l_a, 0.0f);
-        if (ok_b) a.stat[at + g + 8] = make_float4(m_b, M_b, l_b, 0.0f);
-      }
+    if (!whole) {
+      end.flags |= begins ? QR_TAIL : kt + tiles == cur.L ? QR_FRONT | QR_FRONT_ENDS : QR_FRONT;
+      end.rows = min(kRows, rows_all - row0);  // of the last cut unit: the tail's, or a front that fills the share
+      if (!begins) end.front_rows = end.rows;
       if (begins) {
-        owner = make_int4(min(kQrRows, rows_all - t * kQrRows), r, t, h);  // rows, request, row tile, head
-        owner2.x = qa_owner(total, workers, x - kt + L - 1);
+        end.r = cur.r;
+        end.t = cur.t;
+        end.h = cur.h;
+        end.last = qa_owner(total, ctas, x + cur.L - 1);
       }
     }
-    x += tiles;
-    kt = 0;
-    if (x < x_end && ++h == a.heads) {
-      h = 0;
-      ++t;
-      if (t * kQrRows >= rq.n * a.group) {
-        t = 0;
-        do rq = cache_request(a, ++r);
-        while (rq.n == 0);
-      }
-      L = qa_tiles<kQrRows, kQrTile>(a, rq, t);
+    x = tiles_nxt > 0 ? x + tiles + kQaUnitCost : x_end;
+    if (x < x_end && !failed) {
+      seq_used += entries;
+      issued -= min(issued, static_cast<uint32_t>(entries));
+      cur = nxt;
+      tiles = tiles_nxt;
+      kt = 0;
+      now = ahead;
     }
   }
-  if (lane == 0) {
-    a.desc[me * 2] = owner;
-    a.desc[me * 2 + 1] = owner2;
-  }
-  if (failed)  // the copies still under way land (bounded waits) before the shared memory is given up
-    for (uint32_t e = issued > Cfg::kSlots ? issued - Cfg::kSlots : 0; e < issued; ++e)
+  if (failed) {  // the copies still under way land (bounded waits) before the shared memory is given up
+    const uint32_t all = seq_used + issued;
+    for (uint32_t e = all > Cfg::kSlots ? all - Cfg::kSlots : 0; e < all; ++e)
       mbar_wait(&full[e % Cfg::kSlots], (e / Cfg::kSlots) & 1);
+  }
+
+  // ---- the CTA joins the parts that its warps' borders cut: a chain is the tail of one warp, or the front of the
+  // first, and the fronts behind it up to the one that ends the unit. Items (chain, row) are dealt to the warps.
+  if (lane == 0) ends[warp] = end;
+  __syncthreads();
+  int item = 0;
+  for (int s = -1; s < Cfg::kWarps; ++s) {
+    // chain s: begins with warp s's tail, -1: with the front of the CTA's first busy warp
+    int w = s, rows;
+    bool done = false;
+    if (s < 0) {
+      for (w = 0; w < Cfg::kWarps && !ends[w].busy; ++w) {}
+      if (w == Cfg::kWarps || !(ends[w].flags & QR_FRONT)) continue;
+      rows = ends[w].front_rows;
+      done = ends[w].flags & QR_FRONT_ENDS;
+    } else {
+      if (!(ends[w].flags & QR_TAIL)) continue;
+      rows = ends[w].rows;
+    }
+    int last = w;
+    for (int v = w + 1; v < Cfg::kWarps && !done; ++v)
+      if (ends[v].flags & QR_FRONT) {
+        last = v;
+        done = ends[v].flags & QR_FRONT_ENDS;
+      }
+    for (int row = 0; row < rows; ++row, ++item) {
+      if (item % Cfg::kWarps != warp) continue;
+      auto slot = [&](int v) {
+        return (static_cast<int64_t>(blockIdx.x * Cfg::kWarps + v) * 2 + (v == s ? 1 : 0)) * kRows + row;
+      };
+      const bool has = lane >= w && lane <= last && (lane == s || (ends[min(lane, Cfg::kWarps - 1)].flags & QR_FRONT));
+      float4 st = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+      if (has) st = a.stat[slot(lane)];
+      float m = st.x, M = st.y;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+      }
+      const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
+      const float fM = has ? qa_ex2(st.y - Z) : 0.0f;
+      float l = has ? st.z * qa_ex2(st.x - z) : 0.0f;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+      const uint32_t who = __ballot_sync(~0u, has);
+      constexpr int kE = kDim / 32;
+      float acc[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < Cfg::kWarps; ++v) {
+        const float f = __shfl_sync(~0u, fM, v);
+        if (who >> v & 1) {
+          float part[kE];
+          qa_load<kE>(part, a.part + slot(v) * kDim + lane * kE);
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[e] += part[e] * f;
+        }
+      }
+      if (s >= 0 && done) {
+        qa_put<T, kE>(a, ends[s].r, ends[s].t * kRows + row, ends[s].h, lane, z, Z, m, l, acc);
+      } else {
+        const int64_t at = (static_cast<int64_t>(blockIdx.x) * 2 + (s < 0 ? 0 : 1)) * kRows + row;
+        float* dst = a.cta_part + at * kDim + lane * kE;
+#pragma unroll
+        for (int e = 0; e < kE; e += 2) *reinterpret_cast<float2*>(dst + e) = make_float2(acc[e], acc[e + 1]);
+        if (lane == 0) a.cta_stat[at] = make_float4(m, M, l, 0.0f);
+      }
+    }
+    if (s >= 0 && !done && tid == 0)  // cut at the CTA's end: its owner's descriptor
+      a.desc[blockIdx.x] = make_int4(rows | ends[s].last << 8, ends[s].r, ends[s].t, ends[s].h);
+    if (s >= 0 && !done) return;      // the last chain
+  }
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
-// Joins the partial sums of the units that shares cut: the share in which a unit begins names it, its later
-// parts lie in the first slots of the shares up to the last. CTA (eight shares, rows of the tile): a warp joins
-// a unit of up to kQmAlone parts, the whole CTA the longer ones, the parts dealt to its warps; either order
-// is fixed by the shares alone.
+// Joins the parts of the units that CTAs' shares cut: the CTA in which a unit begins names it (tail part), its later
+// parts are the front parts of the CTAs up to the last. CTA (eight owners, rows of the tile): a warp joins a unit of up
+// to kQmAlone parts, the whole CTA the longer ones, their parts dealt to the warps; either order is fixed by the shares.
 constexpr int kQmThreads = 256;
 constexpr int kQmWarps = kQmThreads / 32;
-constexpr int kQmAlone = 16;
+constexpr int kQmAlone = 4;
 
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const CacheAttnArgs a, int shares) {
+__global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const CacheAttnArgs a, int ctas) {
   constexpr int kE = kDim / 32;  // dimensions per lane
   __shared__ float red[kQmWarps][kDim];
-  __shared__ float red_s[kQmWarps][3];
+  __shared__ float red_s[kQmWarps];
   griddep_wait();
-  int row = 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int base = blockIdx.x * kQmWarps;
-  auto slot = [&](int w0, int p) { return (static_cast<int64_t>(w0 + p) * 2 + (p == 0 ? 1 : 0)) * kRows + row; };
-  // sums of the parts p0, p0 + step, ... against the maxima z, Z
-  auto add = [&](int w0, int parts, int p0, int step, float z, float Z, float* acc, float& l) {
-#pragma unroll 4
-    for (int p = p0; p < parts; p += step) {
-      const int64_t at = slot(w0, p);
-      const float4 s = a.stat[at];
-      const float f = qa_ex2(s.y - Z);
-      l += s.z * qa_ex2(s.x - z);
-      const float* src = a.part + at * kDim + lane * kE;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] += src[e] * f;
-    }
-  };
-  auto put = [&](const int4& u, float z, float Z, float m, float l, const float* acc) {
-    const int rr = u.z * kRows + row;
-    const int i = rr / a.group, hq = u.w * a.group + rr - i * a.group;
-    const int64_t out_row = min(max(a.row_start[u.y], 0), a.q_rows) + i;
-    const float n = l == 0.0f ? 0.0f : qa_ex2(Z - z) / l;
-    T* dst = static_cast<T*>(a.out) + out_row * a.out_row + hq * a.out_head + lane * kE;
-#pragma unroll
-    for (int e = 0; e < kE; e += 2) qa_store2<T>(dst + e, acc[e] * n, acc[e + 1] * n);
-    if (lane == 0 && a.lse) a.lse[out_row * a.heads * a.group + hq] = (m + log2f(l)) * 0.6931471805599453f;
-  };
-  auto maxima = [&](int w0, int parts, int p0, int step, float& m, float& M) {
-    for (int p = p0; p < parts; p += step) {
-      const float4 s = a.stat[slot(w0, p)];
-      m = fmaxf(m, s.x);
-      M = fmaxf(M, s.y);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-      M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    }
-  };
-  for (row = blockIdx.y; row < kRows; row += gridDim.y) {
-    if (base + warp < shares) {
-      const int w0 = base + warp;
-      const int4 u = a.desc[w0 * 2];
-      const int parts = row < u.x ? a.desc[w0 * 2 + 1].x - w0 + 1 : 0;
-      if (parts > 0 && parts <= kQmAlone) {
-        float m = -INFINITY, M = -INFINITY, l = 0.0f, acc[kE];
-#pragma unroll
-        for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
-        maxima(w0, parts, lane, 32, m, M);
-        const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
-        add(w0, parts, 0, 1, z, Z, acc, l);
-        put(u, z, Z, m, l, acc);
+  int4 mine = make_int4(0, 0, 0, 0);  // lane i of every warp holds owner base + i
+  if (lane < kQmWarps && base + lane < ctas) mine = a.desc[base + lane];
+  const int my_parts = (mine.x >> 8) - (base + lane) + 1, my_rows = mine.x & 255;
+  for (int row = blockIdx.y; row < kRows; row += gridDim.y) {
+    const uint32_t alone = __ballot_sync(~0u, row < my_rows && my_parts <= kQmAlone);
+    uint32_t many = __ballot_sync(~0u, row < my_rows && my_parts > kQmAlone);
+    if ((alone | many) == 0) return;  // later rows have no owner either
+    auto slot = [&](int c0, int p) { return (static_cast<int64_t>(c0 + p) * 2 + (p == 0 ? 1 : 0)) * kRows + row; };
+    auto maxima = [&](int c0, int parts, int p0, int step, float& m, float& M) {
+      for (int p = p0; p < parts; p += step) {
+        const float4 s = a.cta_stat[slot(c0, p)];
+        m = fmaxf(m, s.x);
+        M = fmaxf(M, s.y);
       }
-    }
-    for (int w0 = base; w0 < min(base + kQmWarps, shares); ++w0) {
-      const int4 u = a.desc[w0 * 2];
-      const int parts = row < u.x ? a.desc[w0 * 2 + 1].x - w0 + 1 : 0;
-      if (parts <= kQmAlone) continue;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+      }
+    };
+    // sums of the parts p0, p0 + step, ... against the maxima z, Z
+    auto add = [&](int c0, int parts, int p0, int step, float z, float Z, float* acc, float& l) {
+#pragma unroll 4
+      for (int p = p0; p < parts; p += step) {
+        const int64_t at = slot(c0, p);
+        const float4 s = a.cta_stat[at];
+        float part[kE];
+        qa_load<kE>(part, a.cta_part + at * kDim + lane * kE);
+        const float f = qa_ex2(s.y - Z);
+        l += s.z * qa_ex2(s.x - z);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) acc[e] += part[e] * f;
+      }
+    };
+    if (alone >> warp & 1) {
+      const int parts = __shfl_sync(~0u, my_parts, warp);
       float m = -INFINITY, M = -INFINITY, l = 0.0f, acc[kE];
 #pragma unroll
       for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
-      maxima(w0, parts, tid, kQmThreads, m, M);
-      __syncthreads();  // the last unit's sums have been read
-      if (lane == 0) {
-        red_s[warp][0] = m;
-        red_s[warp][1] = M;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kQmWarps; ++i) {
-        m = fmaxf(m, red_s[i][0]);
-        M = fmaxf(M, red_s[i][1]);
-      }
+      maxima(base + warp, parts, lane, 32, m, M);
       const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
-      add(w0, parts, warp, kQmWarps, z, Z, acc, l);
+      add(base + warp, parts, 0, 1, z, Z, acc, l);
+      qa_put<T, kE>(a, __shfl_sync(~0u, mine.y, warp), __shfl_sync(~0u, mine.z, warp) * kRows + row,
+                    __shfl_sync(~0u, mine.w, warp), lane, z, Z, m, l, acc);
+    }
+    for (; many; many &= many - 1) {
+      const int i = __ffs(many) - 1;
+      const int parts = __shfl_sync(~0u, my_parts, i);
+      float m = -INFINITY, M = -INFINITY, l = 0.0f, acc[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
+      maxima(base + i, parts, lane, 32, m, M);  // by every warp for itself: the parts are at most one per SM
+      const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
+      add(base + i, parts, warp, kQmWarps, z, Z, acc, l);
+      __syncthreads();  // the last unit's sums have been read
 #pragma unroll
       for (int e = 0; e < kE; ++e) red[warp][lane * kE + e] = acc[e];
-      if (lane == 0) red_s[warp][2] = l;
+      if (lane == 0) red_s[warp] = l;
       __syncthreads();
       if (warp == 0) {
         l = 0.0f;
@@ -666,11 +860,12 @@ __global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const Cach
         for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
 #pragma unroll
         for (int w = 0; w < kQmWarps; ++w) {
-          l += red_s[w][2];
+          l += red_s[w];
 #pragma unroll
           for (int e = 0; e < kE; ++e) acc[e] += red[w][lane * kE + e];
         }
-        put(u, z, Z, m, l, acc);
+        qa_put<T, kE>(a, __shfl_sync(~0u, mine.y, i), __shfl_sync(~0u, mine.z, i) * kRows + row,
+                      __shfl_sync(~0u, mine.w, i), lane, z, Z, m, l, acc);
       }
     }
   }

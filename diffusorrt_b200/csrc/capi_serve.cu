@@ -197,28 +197,48 @@ extern "C" int drt_cache_read(const int32_t* slots, int32_t rows, const void* k_
 namespace {
 constexpr size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// Scratch of a call: partial sums, their statistics and the cut units' descriptors, for every share.
-size_t attend_bytes(int shares, int tile_rows, int dim) {
-  return up256(static_cast<size_t>(shares) * 2 * tile_rows * dim * 4) + up256(static_cast<size_t>(shares) * 2 * tile_rows * 16) +
-         up256(static_cast<size_t>(shares) * 2 * 16);
+// Lays a call's scratch out from `base` and returns its size: the cut units' parts of every warp and CTA.
+size_t attend_scratch(int sms, int dim, uint8_t* base, CacheAttnArgs* a) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = base + at;
+    at += up256(bytes);
+    return p;
+  };
+  const size_t warp_rows = static_cast<size_t>(sms) * kQrMaxParts, cta_rows = static_cast<size_t>(sms) * 2 * kQrMaxRows;
+  a->part = reinterpret_cast<float*>(take(warp_rows * dim * 4));
+  a->stat = reinterpret_cast<float4*>(take(warp_rows * 16));
+  a->cta_part = reinterpret_cast<float*>(take(cta_rows * dim * 4));
+  a->cta_stat = reinterpret_cast<float4*>(take(cta_rows * 16));
+  a->desc = reinterpret_cast<int4*>(take(static_cast<size_t>(sms) * 16));
+  return at;
 }
 
-template <typename T, int kDim, int kCode>
-cudaError_t run_rows(const CacheAttnArgs& a, int device, int grid, int merge_rows, cudaStream_t st) {
-  const size_t smem = QrCfg<kDim>::kSmem;
-  cudaError_t e = allow_smem<cache_attn_rows_kernel<T, kDim, kCode>>(device, smem);
-  if (e == cudaSuccess) e = launch(cache_attn_rows_kernel<T, kDim, kCode>, dim3(grid), dim3(kQrThreads), smem, st, false, a);
+template <typename T, int kDim, int kCode, int kNT>
+cudaError_t run_rows_nt(const CacheAttnArgs& a, int device, int64_t tiles, int sms, int merge_rows, cudaStream_t st) {
+  using Cfg = QrCfg<kDim, kNT>;
+  const int grid = static_cast<int>(std::min<int64_t>(sms, tiles));
+  cudaError_t e = allow_smem<cache_attn_rows_kernel<T, kDim, kCode, kNT>>(device, Cfg::kSmem);
+  if (e == cudaSuccess)
+    e = launch(cache_attn_rows_kernel<T, kDim, kCode, kNT>, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, st, false, a);
   if (e != cudaSuccess || merge_rows == 0) return e;
-  const int shares = grid * kQrWarps;
-  return launch(cache_attn_merge_kernel<T, kDim, kQrRows>, dim3((shares + kQmWarps - 1) / kQmWarps, merge_rows),
-                dim3(kQmThreads), 0, st, true, a, shares);
+  return launch(cache_attn_merge_kernel<T, kDim, Cfg::kRows>,
+                dim3((grid + kQmWarps - 1) / kQmWarps, std::min(merge_rows, Cfg::kRows)), dim3(kQmThreads), 0, st, true, a, grid);
+}
+
+// Eight rows to a tile where the caller's bound says that a kv head's rows fit, else sixteen.
+template <typename T, int kDim, int kCode>
+cudaError_t run_rows(const CacheAttnArgs& a, int device, int64_t rows, int64_t tiles, int sms, int merge_rows, cudaStream_t st) {
+  return rows <= 8 ? run_rows_nt<T, kDim, kCode, 1>(a, device, tiles, sms, merge_rows, st)
+                   : run_rows_nt<T, kDim, kCode, 2>(a, device, tiles, sms, merge_rows, st);
 }
 }  // namespace
 
 extern "C" size_t drt_cache_attend_scratch_bytes(int32_t dim) {
   int device = 0;
   const int sms = current_sms(&device);
-  return attend_bytes((sms > 0 ? sms : 148) * kQrWarps, kQrRows, dim);
+  CacheAttnArgs a;
+  return attend_scratch(sms > 0 ? sms : 148, dim, nullptr, &a);
 }
 
 extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
@@ -267,23 +287,17 @@ extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
   a.out_head = p->out_head;
   a.lse = p->lse;
   a.vec = aligned16(p->q) && (p->q_row | p->q_head) % 8 == 0;
-  const int shares = sms * kQrWarps;
-  uint8_t* s = static_cast<uint8_t*>(p->scratch);
-  a.part = reinterpret_cast<float*>(s);
-  s += up256(static_cast<size_t>(shares) * 2 * kQrRows * p->dim * 4);
-  a.stat = reinterpret_cast<float4*>(s);
-  s += up256(static_cast<size_t>(shares) * 2 * kQrRows * 16);
-  a.desc = reinterpret_cast<int4*>(s);
+  attend_scratch(sms, p->dim, static_cast<uint8_t*>(p->scratch), &a);
   const int max_rows = p->max_rows > 0 ? std::min(p->max_rows, p->q_rows) : p->q_rows;
   // A unit's key tiles at most: with one there is nothing to cut and nothing to join.
   const int64_t deep = (static_cast<int64_t>(p->width) * p->block + kQrTile - 1) / kQrTile;
-  const int64_t units = (static_cast<int64_t>(p->q_rows) * a.group / kQrRows + p->requests) * a.heads;
-  const int grid = static_cast<int>(std::min<int64_t>(sms, units * deep));
-  const int merge_rows = deep > 1 ? static_cast<int>(std::min<int64_t>(kQrRows, static_cast<int64_t>(max_rows) * a.group)) : 0;
+  const int64_t units = (static_cast<int64_t>(p->q_rows) * a.group / 8 + p->requests) * a.heads;
+  const int64_t rows = static_cast<int64_t>(max_rows) * a.group;
+  const int merge_rows = deep > 1 ? static_cast<int>(std::min<int64_t>(kQrMaxRows, rows)) : 0;
   const int dim = p->dim, code = p->code;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CK(p->dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_rows, __nv_bfloat16, a, device, grid, merge_rows, st)
-                               : DRT_DISPATCH_DIM_CODE(run_rows, __half, a, device, grid, merge_rows, st));
+  CK(p->dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_rows, __nv_bfloat16, a, device, rows, units * deep, sms, merge_rows, st)
+                               : DRT_DISPATCH_DIM_CODE(run_rows, __half, a, device, rows, units * deep, sms, merge_rows, st));
   return DRT_OK;
 }
 

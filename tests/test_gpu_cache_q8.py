@@ -400,6 +400,14 @@ def test_attend_long_axis_is_split_and_joined(kernels):
         check_attend(kernels, attend_case(15, requests, 4, 2, 64, 64, I8, BF), max_rows=2)
 
 
+@pytest.mark.parametrize("dim,code,heads,rows", [(128, E4, 16, 1), (64, I8, 16, 1), (128, I8, 40, 1), (128, E4, 32, 5)])
+def test_attend_many_units_and_tiles_to_a_share(kernels, dim, code, heads, rows):
+    """More work than the GPU has warps: each goes through several units, of one tile and of many."""
+    rng = random.Random(dim + heads)
+    requests = [(rng.choice([1, rows]), rng.choice([0, 3, 64, 65, 200, 700, 1400])) for _ in range(120)]
+    check_attend(kernels, attend_case(21, requests, heads, 16 if heads < 32 else 8, dim, 64, code, BF), max_rows=rows)
+
+
 @pytest.mark.parametrize("mask_block", [0, 1, 32])
 @pytest.mark.parametrize("dim,code,typ", [(128, I8, BF), (128, E4, HF), (64, E4, BF), (64, I8, HF)])
 def test_attend_many_rows(kernels, mask_block, dim, code, typ):
