@@ -182,7 +182,7 @@ SIGNATURES = {
                                         _I32, _I32, _P]),
     "drt_cache_read": (ctypes.c_int, [_P, _I32, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _P]),
     "drt_cache_attend_scratch_bytes": (ctypes.c_size_t, [_I32]),
-    "drt_cache_attend": (ctypes.c_int, [ctypes.POINTER(CacheAttendArgs), _P]),
+    "drt_cache_attend": (ctypes.c_int, [_P, _P]),  # the address or bytes of a CacheAttendArgs
     "drt_selector_logprobs_scratch_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
     "drt_selector_logprobs": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I32, _P, ctypes.c_double, _I32, _I32, _P, _P, _P,
                                              _P, _P, _P, _P]),

@@ -190,14 +190,21 @@ __device__ __forceinline__ void qa_next(const CacheAttnArgs& a, QaUnit& u) {
   qa_size<kRows, kTile>(a, u);
 }
 
-__device__ __forceinline__ int64_t qa_share(int64_t total, int shares, int w) { return total * w / shares; }
-// The share that holds tile x.
-__device__ __forceinline__ int qa_owner(int64_t total, int shares, int64_t x) {
-  int w = static_cast<int>(x * shares / total);
-  while (w + 1 < shares && qa_share(total, shares, w + 1) <= x) ++w;
-  while (w > 0 && qa_share(total, shares, w) > x) --w;
-  return w;
-}
+// The axis of `total` places cut into `shares`: each has `each` places, the first `more` of them one more.
+struct QaCut {
+  int64_t each;
+  int more;
+  __device__ __forceinline__ QaCut(int64_t total, int shares) {
+    each = total >> 31 ? total / shares : static_cast<uint32_t>(total) / static_cast<uint32_t>(shares);
+    more = static_cast<int>(total - each * shares);
+  }
+  __device__ __forceinline__ int64_t begin(int w) const { return each * w + min(w, more); }
+  // The share that holds place x.
+  __device__ __forceinline__ int owner(int64_t x) const {
+    const int64_t wide = (each + 1) * more;
+    return static_cast<int>(x < wide ? x / (each + 1) : more + (x - wide) / each);
+  }
+};
 
 // What a unit costs beside its tiles, in tiles: the reads of its queries and table, its softmax's start and its output.
 // A unit takes so many places on the axis before its first tile, so that the shares of many short units are not
@@ -308,16 +315,24 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
     for (int i = 0; i < Cfg::kSlots; ++i) mbar_init(&full[i], 1);
   fence_mbar_init();
 
+  griddep_launch_dependents();  // the join's CTAs may take what is left of the SMs; they wait for this grid's end
+  // the table entries on their way to L2 while the lengths are read
+  for (int64_t i = blockIdx.x * Cfg::kThreads + tid; i * 32 < static_cast<int64_t>(a.requests) * a.width && i < 65536;
+       i += gridDim.x * Cfg::kThreads) {
+    const int64_t e = i * 32, r = e / a.width;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.tables + r * a.ld_tables + (e - r * a.width)));
+  }
   __shared__ QrEnd ends[Cfg::kWarps];
   int64_t* prefix = reinterpret_cast<int64_t*>(qr_smem);
   const int64_t total = qa_prefix<kRows, kQrTile, Cfg::kThreads>(a, prefix);
   const int ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
   int64_t x = 0, x_end = 0;
   QaUnit cur = {};
+  const QaCut cut(total, max(ctas, 1));
   if (blockIdx.x < ctas) {
-    const int64_t c0 = qa_share(total, ctas, blockIdx.x), n = qa_share(total, ctas, blockIdx.x + 1) - c0;
-    x = c0 + qa_share(n, Cfg::kWarps, warp);
-    x_end = c0 + qa_share(n, Cfg::kWarps, warp + 1);
+    const int64_t c0 = cut.begin(blockIdx.x), n = cut.begin(blockIdx.x + 1) - c0;
+    x = c0 + n * warp / Cfg::kWarps;
+    x_end = c0 + n * (warp + 1) / Cfg::kWarps;
     int hi = a.requests;
     while (hi - cur.r > 1) {
       const int mid = (cur.r + hi) >> 1;
@@ -342,8 +357,9 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
       ++cur.t;
       qa_size<kRows, kQrTile>(a, cur);
     }
-    cur.h = static_cast<int>(rem / (cur.L + kQaUnitCost));
-    kt = static_cast<int>(rem % (cur.L + kQaUnitCost)) - kQaUnitCost;
+    const int per = cur.L + kQaUnitCost;
+    cur.h = rem >> 31 ? static_cast<int>(rem / per) : static_cast<int>(rem) / per;
+    kt = static_cast<int>(rem - static_cast<int64_t>(cur.h) * per) - kQaUnitCost;
     if (kt < 0) {            // the share begins before the unit's first tile
       x -= kt;
       kt = 0;
@@ -686,7 +702,7 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
         end.r = cur.r;
         end.t = cur.t;
         end.h = cur.h;
-        end.last = qa_owner(total, ctas, x + cur.L - 1);
+        end.last = cut.owner(x + cur.L - 1);
       }
     }
     x = tiles_nxt > 0 ? x + tiles + kQaUnitCost : x_end;
@@ -735,6 +751,12 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
         return (static_cast<int64_t>(blockIdx.x * Cfg::kWarps + v) * 2 + (v == s ? 1 : 0)) * kRows + row;
       };
       const bool has = lane >= w && lane <= last && (lane == s || (ends[min(lane, Cfg::kWarps - 1)].flags & QR_FRONT));
+      const uint32_t who = __ballot_sync(~0u, has);
+      constexpr int kE = kDim / 32;
+      float part[Cfg::kWarps][kE];
+#pragma unroll
+      for (int v = 0; v < Cfg::kWarps; ++v)  // all loads at once; a warp without a part gives the first one's, times 0
+        qa_load<kE>(part[v], a.part + slot(who >> v & 1 ? v : w) * kDim + lane * kE);
       float4 st = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
       if (has) st = a.stat[slot(lane)];
       float m = st.x, M = st.y;
@@ -748,20 +770,14 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
       float l = has ? st.z * qa_ex2(st.x - z) : 0.0f;
 #pragma unroll
       for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
-      const uint32_t who = __ballot_sync(~0u, has);
-      constexpr int kE = kDim / 32;
       float acc[kE];
 #pragma unroll
       for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
 #pragma unroll
       for (int v = 0; v < Cfg::kWarps; ++v) {
         const float f = __shfl_sync(~0u, fM, v);
-        if (who >> v & 1) {
-          float part[kE];
-          qa_load<kE>(part, a.part + slot(v) * kDim + lane * kE);
 #pragma unroll
-          for (int e = 0; e < kE; ++e) acc[e] += part[e] * f;
-        }
+        for (int e = 0; e < kE; ++e) acc[e] += part[v][e] * f;
       }
       if (s >= 0 && done) {
         qa_put<T, kE>(a, ends[s].r, ends[s].t * kRows + row, ends[s].h, lane, z, Z, m, l, acc);
@@ -781,9 +797,9 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
 }
 
 // Joins the parts of the units that CTAs' shares cut: the CTA in which a unit begins names it (tail part), its later
-// parts are the front parts of the CTAs up to the last. CTA (eight owners, rows of the tile): a warp joins a unit of up
+// parts are the front parts of the CTAs up to the last. CTA (four owners, rows of the tile): a warp joins a unit of up
 // to kQmAlone parts, the whole CTA the longer ones, their parts dealt to the warps; either order is fixed by the shares.
-constexpr int kQmThreads = 256;
+constexpr int kQmThreads = 128;  // with their registers they fit beside a CTA of the rows kernel
 constexpr int kQmWarps = kQmThreads / 32;
 constexpr int kQmAlone = 4;
 
@@ -817,7 +833,7 @@ __global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const Cach
     };
     // sums of the parts p0, p0 + step, ... against the maxima z, Z
     auto add = [&](int c0, int parts, int p0, int step, float z, float Z, float* acc, float& l) {
-#pragma unroll 4
+#pragma unroll 5
       for (int p = p0; p < parts; p += step) {
         const int64_t at = slot(c0, p);
         const float4 s = a.cta_stat[at];

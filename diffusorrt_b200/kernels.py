@@ -7,8 +7,8 @@ the token scorer (select_logprobs).
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -209,38 +209,63 @@ def linear_q4(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, bias: torch
 
 
 # ------------------------------------------------------------------ batch serving: paged 8-bit cache, token scores
+# These run once or more per layer and step, so their host path is kept short: attributes are read once, messages
+# are built only when a check fails, and outputs of one type share an allocation.
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 _CODES = {torch.int8: _lib.CODE_INT8, torch.float8_e4m3fn: _lib.CODE_E4M3}
+_I32 = torch.int32
+_ATTEND = struct.Struct("@PqqPqq5PqPq4P11if")  # CacheAttendArgs
+_scratch_bytes: dict[tuple[int, int], int] = {}
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
+def _check_ints(t, name: str, index: int, n: int | None = None) -> None:
+    """t is a contiguous int32 vector (of n entries) on device `index` (-1: the CPU)."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is _I32 and t.get_device() == index and t.dim() == 1
+            and t.is_contiguous() and (n is None or t.numel() == n)):
+        raise ValueError(f"{name} must be a contiguous int32 vector{'' if n is None else f' of {n} entries'} on "
+                         f"{'the CPU' if index < 0 else f'cuda:{index}'}")
 
 
-def _ints(t: torch.Tensor, name: str, device, shape: tuple[int, ...] | None = None) -> torch.Tensor:
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.is_contiguous()
-          and (t.dim() == 1 if shape is None else tuple(t.shape) == shape),
-          f"{name} must be a contiguous int32 tensor{'' if shape is None else f' of shape {shape}'} on {device}")
-    return t
+def _check_tables(t, index: int, n: int) -> tuple[int, int]:
+    """(width, row stride) of the block tables."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is _I32 and t.get_device() == index and t.dim() == 2 and t.size(0) == n
+            and t.stride(1) == 1 and (n <= 1 or t.stride(0) >= t.size(1))):
+        raise ValueError(f"tables must be an int32 [{n}, width] tensor with contiguous rows on cuda:{index}")
+    width = t.size(1)
+    return width, max(t.stride(0), width)
 
 
-def _launch(device, stream: torch.cuda.Stream | None, made: list, call) -> None:
-    """call(stream pointer) with `device` current. Tensors made here are allocated on the current stream;
-    the allocator is told when the work runs on another one."""
-    with torch.cuda.device(device):
-        current = torch.cuda.current_stream(device)
-        use = stream if stream is not None else current
-        _need(use.device == device, f"the stream belongs to {use.device}, the tensors to {device}")
-        if use != current and made:
-            use.wait_stream(current)  # memory that the allocator hands out may still be in use there
+def _launch(index: int, stream: torch.cuda.Stream | None, made, fn, *args) -> None:
+    """fn(*args, stream) with device `index` current. Tensors made for the call belong to the current stream; when
+    the work runs on another one, that waits for it and the allocator is told."""
+    if stream is None:
+        if torch.cuda.current_device() == index:
+            _lib.check(fn(*args, _current_stream(index)))
+        else:
+            with torch.cuda.device(index):
+                _lib.check(fn(*args, _current_stream(index)))
+        return
+    if stream.device.index != index:
+        raise ValueError(f"the stream belongs to {stream.device}, the tensors to cuda:{index}")
+    with torch.cuda.device(index):
+        current = torch.cuda.current_stream(index)
+        if stream != current and made:
+            stream.wait_stream(current)  # memory that the allocator hands out may still be in use there
             for t in made:
-                t.record_stream(use)
-        _lib.check(call(int(use.cuda_stream)))
+                t.record_stream(stream)
+        _lib.check(fn(*args, int(stream.cuda_stream)))
+
+
+def _current_stream(index: int) -> int:
+    return int(torch.cuda.current_stream(index).cuda_stream)
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _current_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811  (the same without a Stream object)
 
 
 class CachePlan(NamedTuple):
-    """A step's slot maps (all int32): row r of the batch is rows row_start[r] .. row_start[r + 1]."""
+    """A step's slot maps (all int32): request r's rows in the batch are row_start[r] .. row_start[r + 1]."""
 
     row_start: torch.Tensor   # [requests + 1]
     slots: torch.Tensor       # [max_rows], -1 behind the last row
@@ -261,53 +286,66 @@ def plan_cache(start: torch.Tensor, count: torch.Tensor, held: torch.Tensor, tab
     are ring_state[1] entries from ring_state[0] on. tables and ring are updated in place; held and
     ring_state too, unless their _out tensors are other ones. A call that cannot be served changes nothing
     and says why in `status` (drt_cache_plan)."""
-    _need(isinstance(start, torch.Tensor) and start.is_cuda, "start must be a CUDA tensor")
-    dev = start.device
-    _ints(start, "start", dev)
-    n = start.numel()
-    _ints(count, "count", dev, (n,))
-    _ints(held, "held", dev, (n,))
-    _ints(ring, "ring", dev)
-    _ints(ring_state, "ring_state", dev, (2,))
-    _need(isinstance(tables, torch.Tensor) and tables.dtype == torch.int32 and tables.device == dev and tables.dim() == 2
-          and tables.shape[0] == n and tables.stride(1) == 1 and (n <= 1 or tables.stride(0) >= tables.shape[1]),
-          f"tables must be an int32 [{n}, width] tensor with contiguous rows on {dev}")
-    _need(max_rows >= 0, "max_rows must be >= 0")
-    held_out = held if held_out is None else _ints(held_out, "held_out", dev, (n,))
-    ring_state_out = ring_state if ring_state_out is None else _ints(ring_state_out, "ring_state_out", dev, (2,))
-    out = [torch.empty(m, dtype=torch.int32, device=dev) for m in (n + 1, max_rows, max_rows, n, 1)]
-    row_start, slots, positions, lengths, status = out
-    width = tables.shape[1]
-    _launch(dev, stream, out, lambda s: _lib.load().drt_cache_plan(
-        start.data_ptr(), count.data_ptr(), held.data_ptr(), held_out.data_ptr(), n, tables.data_ptr(),
-        max(tables.stride(0), width), width, int(block_size), ring.data_ptr(), ring.numel(), ring_state.data_ptr(),
-        ring_state_out.data_ptr(), row_start.data_ptr(), slots.data_ptr(), positions.data_ptr(), int(max_rows),
-        lengths.data_ptr(), status.data_ptr(), s))
+    if not (isinstance(start, torch.Tensor) and start.is_cuda):
+        raise ValueError("start must be a CUDA tensor")
+    index, n = start.get_device(), start.numel()
+    _check_ints(start, "start", index)
+    _check_ints(count, "count", index, n)
+    _check_ints(held, "held", index, n)
+    _check_ints(ring, "ring", index)
+    _check_ints(ring_state, "ring_state", index, 2)
+    width, ld = _check_tables(tables, index, n)
+    if max_rows < 0:
+        raise ValueError("max_rows must be >= 0")
+    if held_out is None:
+        held_out = held
+    else:
+        _check_ints(held_out, "held_out", index, n)
+    if ring_state_out is None:
+        ring_state_out = ring_state
+    else:
+        _check_ints(ring_state_out, "ring_state_out", index, 2)
+    made = torch.empty(2 * n + 2 * max_rows + 2, dtype=_I32, device=start.device)
+    row_start, slots, positions, lengths, status = made.split((n + 1, max_rows, max_rows, n, 1))
+    p = made.data_ptr()
+    _launch(index, stream, (made,), _lib.load().drt_cache_plan, start.data_ptr(), count.data_ptr(), held.data_ptr(),
+            held_out.data_ptr(), n, tables.data_ptr(), ld, width, block_size, ring.data_ptr(), ring.numel(),
+            ring_state.data_ptr(), ring_state_out.data_ptr(), p, p + 4 * (n + 1), p + 4 * (n + 1 + max_rows), max_rows,
+            p + 4 * (n + 1 + 2 * max_rows), p + 4 * (2 * n + 1 + 2 * max_rows))
     return CachePlan(row_start, slots, positions, lengths, held_out, ring_state_out, status)
 
 
 def cache_q8(blocks: int, kv_heads: int, block_size: int, dim: int = 128, *, dtype: torch.dtype = torch.int8, device="cuda"):
     """A new, empty 8-bit cache: (k_cache, v_cache, k_scale, v_scale) in the layout of the operators below."""
-    _need(dtype in _CODES, "an 8-bit cache holds int8 or float8_e4m3fn")
-    _need(block_size in (16, 32, 64, 128), "a block holds 16, 32, 64 or 128 tokens")
+    if dtype not in _CODES:
+        raise ValueError("an 8-bit cache holds int8 or float8_e4m3fn")
+    if block_size not in (16, 32, 64, 128):
+        raise ValueError("a block holds 16, 32, 64 or 128 tokens")
     k = torch.zeros(blocks, kv_heads, block_size, dim, dtype=torch.int8, device=device).view(dtype)
     v = torch.zeros(blocks, kv_heads, block_size // 16, dim, 16, dtype=torch.int8, device=device).view(dtype)
     scale = torch.zeros(2, blocks, kv_heads, dtype=torch.float32, device=device)
     return k, v, scale[0], scale[1]
 
 
-def _cache_args(k_cache, v_cache, k_scale, v_scale, device):
-    """(blocks, kv_heads, block, dim, code) of a cache on `device`."""
-    _need(all(isinstance(t, torch.Tensor) and t.device == device and t.is_contiguous()
-              for t in (k_cache, v_cache, k_scale, v_scale)), f"the cache must be contiguous tensors on {device}")
-    _need(k_cache.dtype in _CODES and v_cache.dtype == k_cache.dtype, "k_cache and v_cache must be int8 or float8_e4m3fn")
-    _need(k_cache.dim() == 4, "k_cache must be [blocks, kv_heads, block, dim]")
+def _cache_args(k_cache, v_cache, k_scale, v_scale, index: int):
+    """(blocks, kv_heads, block, dim, code) of a cache on device `index`."""
+    if not all(isinstance(t, torch.Tensor) and t.get_device() == index and t.is_contiguous()
+               for t in (k_cache, v_cache, k_scale, v_scale)):
+        raise ValueError(f"the cache must be contiguous tensors on {'the CPU' if index < 0 else f'cuda:{index}'}")
+    code = _CODES.get(k_cache.dtype)
+    if code is None or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("k_cache and v_cache must be int8 or float8_e4m3fn")
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [blocks, kv_heads, block, dim]")
     blocks, heads, block, dim = k_cache.shape
-    _need(block in (16, 32, 64, 128), "a block holds 16, 32, 64 or 128 tokens")
-    _need(tuple(v_cache.shape) == (blocks, heads, block // 16, dim, 16), "v_cache must be [blocks, kv_heads, block / 16, dim, 16]")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        _need(t.dtype == torch.float32 and tuple(t.shape) == (blocks, heads), f"{name} must be float32 [blocks, kv_heads]")
-    return blocks, heads, block, dim, _CODES[k_cache.dtype]
+    if block not in (16, 32, 64, 128):
+        raise ValueError("a block holds 16, 32, 64 or 128 tokens")
+    if v_cache.shape != (blocks, heads, block // 16, dim, 16):
+        raise ValueError("v_cache must be [blocks, kv_heads, block / 16, dim, 16]")
+    shape = (blocks, heads)
+    if k_scale.shape != shape or v_scale.shape != shape or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
+        raise ValueError("k_scale and v_scale must be float32 [blocks, kv_heads]")
+    return blocks, heads, block, dim, code
 
 
 def append_cache_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -317,41 +355,60 @@ def append_cache_q8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cac
     A block's scale covers its tokens: it grows with the largest value appended (the tokens already there are
     rounded anew), and a run of rows that begins a block starts it anew. Rows whose slot is -1 are skipped;
     slots are distinct and those of one block consecutive rows, as plan_cache gives them."""
-    _need(isinstance(k, torch.Tensor) and k.is_cuda and k.dim() == 3, "k must be a CUDA tensor [rows, kv_heads, dim]")
-    dev = k.device
-    blocks, heads, block, dim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, dev)
-    rows = k.shape[0]
-    for name, t in (("k", k), ("v", v)):
-        _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype == k.dtype and tuple(t.shape) == (rows, heads, dim)
-              and t.stride(2) == 1, f"{name} must be [rows, {heads}, {dim}] with a contiguous last dimension on {dev}")
-    _need(k.dtype in (torch.bfloat16, torch.float16), "k and v must be bf16 or f16")
-    _ints(slots, "slots", dev)
-    _need(slots.numel() >= rows, "one slot per row")
-    _launch(dev, stream, [], lambda s: _lib.load().drt_cache_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _TYPES[k.dtype], rows,
-        slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads,
-        block, dim, code, s))
+    if not (isinstance(k, torch.Tensor) and k.is_cuda and k.dim() == 3):
+        raise ValueError("k must be a CUDA tensor [rows, kv_heads, dim]")
+    index = k.get_device()
+    blocks, heads, block, dim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, index)
+    shape, dtype = k.shape, k.dtype
+    rows = shape[0]
+    if not (isinstance(v, torch.Tensor) and v.get_device() == index and v.dtype is dtype and v.shape == shape
+            and shape[1] == heads and shape[2] == dim):
+        raise ValueError(f"k and v must be [rows, {heads}, {dim}] of one type on cuda:{index}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError("k and v must be bf16 or f16")
+    k_row, k_head, k_dim = k.stride()
+    v_row, v_head, v_dim = v.stride()
+    if k_dim != 1 or v_dim != 1:
+        raise ValueError("k and v must have a contiguous last dimension")
+    _check_ints(slots, "slots", index)
+    if slots.numel() < rows:
+        raise ValueError("one slot per row")
+    _launch(index, stream, (), _lib.load().drt_cache_append, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+            _TYPES[dtype], rows, slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), blocks, heads, block, dim, code)
 
 
 def read_cache_q8(slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, stream: torch.cuda.Stream | None = None):
     """The K and V values of the listed slots, [slots, kv_heads, dim] each, rounded once to dtype (zeros for -1)."""
-    _need(isinstance(slots, torch.Tensor) and slots.is_cuda, "slots must be a CUDA tensor")
-    dev = slots.device
-    _ints(slots, "slots", dev)
-    blocks, heads, block, dim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, dev)
-    _need(dtype in _TYPES, "values are read as bfloat16, float16 or float32")
-    k, v = (torch.empty(slots.numel(), heads, dim, dtype=dtype, device=dev) for _ in range(2))
-    _launch(dev, stream, [k, v], lambda s: _lib.load().drt_cache_read(
-        slots.data_ptr(), slots.numel(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        blocks, heads, block, dim, code, k.data_ptr(), v.data_ptr(), _TYPES[dtype], s))
+    if not (isinstance(slots, torch.Tensor) and slots.is_cuda):
+        raise ValueError("slots must be a CUDA tensor")
+    index = slots.get_device()
+    _check_ints(slots, "slots", index)
+    blocks, heads, block, dim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, index)
+    if dtype not in _TYPES:
+        raise ValueError("values are read as bfloat16, float16 or float32")
+    n = slots.numel()
+    made = torch.empty(2, n, heads, dim, dtype=dtype, device=slots.device)
+    k, v = made.unbind(0)
+    _launch(index, stream, (made,), _lib.load().drt_cache_read, slots.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, block, dim, code, k.data_ptr(), v.data_ptr(), _TYPES[dtype])
     return k, v
+
+
+def _attend_bytes(dim: int, index: int) -> int:
+    size = _scratch_bytes.get((index, dim))
+    if size is None:
+        with torch.cuda.device(index):
+            size = _scratch_bytes[index, dim] = int(_lib.load().drt_cache_attend_scratch_bytes(int(dim)))
+    return size
 
 
 def attend_scratch(dim: int, device) -> torch.Tensor:
     """Scratch of one attend_cache_q8 call in flight (captured graphs that may run at once need one each)."""
-    with torch.cuda.device(device):
-        return torch.empty(int(_lib.load().drt_cache_attend_scratch_bytes(int(dim))), dtype=torch.uint8, device=device)
+    device = torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch.empty(_attend_bytes(dim, index), dtype=torch.uint8, device=torch.device("cuda", index))
 
 
 def attend_cache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -367,47 +424,49 @@ def attend_cache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     0 shows every token. scale defaults to 1 / sqrt(dim). max_rows: a bound on a request's rows, if the
     caller knows one (1 for single-token decoding); it changes speed only. Rows behind the last request's
     are left as they are in `out` and `lse` (new ones: zeros)."""
-    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16)
-          and q.stride(2) == 1, "q must be a bf16 or f16 CUDA tensor [rows, heads, dim] with a contiguous last dimension")
-    dev = q.device
-    rows, heads, dim = q.shape
-    blocks, kv_heads, block, kdim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, dev)
-    _need(dim == kdim and heads % kv_heads == 0, "q and the cache disagree on heads or dim")
-    _ints(lengths, "lengths", dev)
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3):
+        raise ValueError("q must be a CUDA tensor [rows, heads, dim]")
+    index, dtype, shape = q.get_device(), q.dtype, q.shape
+    rows, heads, dim = shape
+    q_row, q_head, q_dim = q.stride()
+    if q_dim != 1 or (dtype is not torch.bfloat16 and dtype is not torch.float16):
+        raise ValueError("q must be bf16 or f16 with a contiguous last dimension")
+    blocks, kv_heads, block, kdim, code = _cache_args(k_cache, v_cache, k_scale, v_scale, index)
+    if dim != kdim or heads % kv_heads != 0:
+        raise ValueError("q and the cache disagree on heads or dim")
+    _check_ints(lengths, "lengths", index)
     n = lengths.numel()
-    _ints(row_start, "row_start", dev, (n + 1,))
-    _need(isinstance(tables, torch.Tensor) and tables.dtype == torch.int32 and tables.device == dev and tables.dim() == 2
-          and tables.shape[0] == n and tables.stride(1) == 1 and (n <= 1 or tables.stride(0) >= tables.shape[1]),
-          f"tables must be an int32 [{n}, width] tensor with contiguous rows on {dev}")
+    _check_ints(row_start, "row_start", index, n + 1)
+    width, ld = _check_tables(tables, index, n)
     if origin is not None:
-        _ints(origin, "origin", dev, (n,))
+        _check_ints(origin, "origin", index, n)
     made = []
     if out is None:
-        out = torch.zeros(rows, heads, dim, dtype=q.dtype, device=dev)
+        out = torch.zeros(rows, heads, dim, dtype=dtype, device=q.device)
         made.append(out)
-    _need(out.dtype == q.dtype and out.device == dev and out.shape == q.shape and out.stride(2) == 1,
-          "out must have q's shape and dtype and a contiguous last dimension")
+    elif not (isinstance(out, torch.Tensor) and out.dtype is dtype and out.get_device() == index and out.shape == shape):
+        raise ValueError("out must have q's shape and dtype on its device")
+    out_row, out_head, out_dim = out.stride()
+    if out_dim != 1:
+        raise ValueError("out must have a contiguous last dimension")
     if lse is None:
-        lse = torch.zeros(rows, heads, dtype=torch.float32, device=dev)
+        lse = torch.zeros(rows, heads, dtype=torch.float32, device=q.device)
         made.append(lse)
-    _need(lse.dtype == torch.float32 and lse.device == dev and tuple(lse.shape) == (rows, heads) and lse.is_contiguous(),
-          "lse must be a contiguous float32 [rows, heads] tensor")
+    elif not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32 and lse.get_device() == index
+              and lse.shape == (rows, heads) and lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [rows, heads] tensor")
+    size = _attend_bytes(dim, index)
     if scratch is None:
-        scratch = attend_scratch(dim, dev)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         made.append(scratch)
-    with torch.cuda.device(dev):
-        _need(scratch.device == dev and scratch.is_contiguous()
-              and scratch.numel() * scratch.element_size() >= _lib.load().drt_cache_attend_scratch_bytes(dim),
-              "scratch is too small (attend_scratch)")
-    args = _lib.CacheAttendArgs(
-        q=q.data_ptr(), q_row=q.stride(0), q_head=q.stride(1), out=out.data_ptr(), out_row=out.stride(0),
-        out_head=out.stride(1), lse=lse.data_ptr(), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
-        k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), blocks=blocks, tables=tables.data_ptr(),
-        ld_tables=max(tables.stride(0), tables.shape[1]), lengths=lengths.data_ptr(), row_start=row_start.data_ptr(),
-        origin=None if origin is None else origin.data_ptr(), scratch=scratch.data_ptr(), q_rows=rows, heads=heads,
-        kv_heads=kv_heads, dim=dim, dtype=_TYPES[q.dtype], code=code, block=block, width=tables.shape[1], requests=n,
-        mask_block=int(mask_block), max_rows=int(max_rows), scale=1 / math.sqrt(dim) if scale is None else float(scale))
-    _launch(dev, stream, made, lambda s: _lib.load().drt_cache_attend(ctypes.byref(args), s))
+    elif not (scratch.get_device() == index and scratch.is_contiguous() and scratch.numel() * scratch.element_size() >= size):
+        raise ValueError("scratch is too small (attend_scratch)")
+    args = _ATTEND.pack(
+        q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, lse.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), blocks, tables.data_ptr(), ld, lengths.data_ptr(), row_start.data_ptr(),
+        0 if origin is None else origin.data_ptr(), scratch.data_ptr(), rows, heads, kv_heads, dim, _TYPES[dtype], code, block,
+        width, n, mask_block, max_rows, 1 / math.sqrt(dim) if scale is None else scale)
+    _launch(index, stream, made, _lib.load().drt_cache_attend, args)
     return out, lse
 
 
@@ -427,30 +486,40 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     """Log probabilities of given tokens (int32) under softmax(logits / T) of f32, bf16 or f16 rows [rows, vocab]
     (or of the rows row_index), with the entropy, the token's rank and the `top` <= 32 likeliest tokens.
     exclude_token counts as a logit of -inf; a token outside the vocabulary scores -inf with rank -1."""
-    _need(isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in _TYPES
-          and logits.stride(1) == 1, "logits must be a row-major CUDA float32, bfloat16 or float16 [rows, vocab] tensor")
-    dev = logits.device
-    _ints(tokens, "tokens", dev)
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2):
+        raise ValueError("logits must be a CUDA tensor [rows, vocab]")
+    index = logits.get_device()
+    typ = _TYPES.get(logits.dtype)
+    ld, step = logits.stride()
+    if typ is None or step != 1:
+        raise ValueError("logits must be row-major float32, bfloat16 or float16")
+    have, vocab = logits.shape
+    _check_ints(tokens, "tokens", index)
     n = tokens.numel()
-    if row_index is None:
-        _need(n == logits.shape[0], "one token per logits row")
+    if row_index is not None:
+        _check_ints(row_index, "row_index", index, n)
+    elif n != have:
+        raise ValueError("one token per logits row")
+    if not 0 <= top <= 32:
+        raise ValueError("top must be in [0, 32]")
+    if torch.cuda.current_device() == index:
+        size = _lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ)
     else:
-        _ints(row_index, "row_index", dev, (n,))
-    _need(0 <= top <= 32, "top must be in [0, 32]")
-    vocab, typ = logits.shape[1], _TYPES[logits.dtype]
-    made = [torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev),
-            torch.empty(n, dtype=torch.int32, device=dev), torch.empty(n, top, dtype=torch.int32, device=dev),
-            torch.empty(n, top, dtype=torch.float32, device=dev)]
-    out = TokenScores(*made)
-    with torch.cuda.device(dev):
-        size = int(_lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ))
-    if scratch is None:
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-        made.append(scratch)
-    _need(scratch.device == dev and scratch.is_contiguous() and scratch.numel() * scratch.element_size() >= size,
-          f"scratch must hold {size} bytes")
-    _launch(dev, stream, made, lambda s: _lib.load().drt_selector_logprobs(
-        logits.data_ptr(), typ, max(logits.stride(0), vocab), None if row_index is None else row_index.data_ptr(), n, vocab,
-        tokens.data_ptr(), float(temperature), int(exclude_token), int(top), scratch.data_ptr(), out.logprob.data_ptr(),
-        out.entropy.data_ptr(), out.rank.data_ptr(), out.top_token.data_ptr(), out.top_logprob.data_ptr(), s))
-    return out
+        with torch.cuda.device(index):
+            size = _lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ)
+    words = n * (3 + 2 * top)
+    # outputs in one allocation, the call's scratch in front of them
+    own = (size + 3) // 4 if scratch is None else 0
+    made = torch.empty(own + words, dtype=torch.float32, device=logits.device)
+    if scratch is not None and not (scratch.get_device() == index and scratch.is_contiguous()
+                                    and scratch.numel() * scratch.element_size() >= size):
+        raise ValueError(f"scratch must hold {size} bytes")
+    _, logprob, entropy, top_logprob, whole = made.split((own, n, n, n * top, n * (1 + top)))
+    rank, top_token = whole.view(_I32).split((n, n * top))
+    p = made.data_ptr()
+    at = p + 4 * own
+    _launch(index, stream, (made,) if scratch is None else (made, scratch), _lib.load().drt_selector_logprobs,
+            logits.data_ptr(), typ, max(ld, vocab), 0 if row_index is None else row_index.data_ptr(), n, vocab,
+            tokens.data_ptr(), temperature, exclude_token, top, p if scratch is None else scratch.data_ptr(), at, at + 4 * n,
+            at + 4 * n * (2 + top), at + 4 * n * (3 + top), at + 8 * n)
+    return TokenScores(logprob, entropy, rank, top_token.view(n, top), top_logprob.view(n, top))

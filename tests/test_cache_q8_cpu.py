@@ -24,7 +24,7 @@ def lib():
 
 
 def test_args_struct_matches_header(tmp_path):
-    from diffusorrt_b200 import _lib
+    from diffusorrt_b200 import _lib, kernels
 
     cc = shutil.which("gcc") or shutil.which("cc")
     if cc is None:
@@ -35,6 +35,7 @@ def test_args_struct_matches_header(tmp_path):
     lines += [f'printf("{f} %zu\\n", offsetof(drt_cache_attend_args, {f}));' for f, _ in py._fields_]
     (tmp_path / "a.c").write_text("\n".join(lines + ["return 0; }"]))
     subprocess.run([cc, "-I", str(ROOT / "include"), str(tmp_path / "a.c"), "-o", str(tmp_path / "a")], check=True)
+    assert kernels._ATTEND.size == ctypes.sizeof(py)
     for line in subprocess.run([str(tmp_path / "a")], check=True, capture_output=True, text=True).stdout.split("\n")[:-1]:
         name, value = line.split()
         assert int(value) == (ctypes.sizeof(py) if name == "size" else getattr(py, name).offset), name
@@ -157,7 +158,7 @@ def test_python_checks_come_before_the_library():
                  lambda: kernels.select_logprobs(torch.zeros(2, 9), slots)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
-    dev = torch.device("cpu")
+    dev = -1  # the CPU
     with pytest.raises(ValueError, match="int8 or float8"):
         kernels._cache_args(cache[0].to(torch.uint8), *cache[1:], dev)
     with pytest.raises(ValueError, match="16, 32, 64 or 128"):
@@ -171,7 +172,7 @@ def test_python_checks_come_before_the_library():
     with pytest.raises(ValueError, match="int8 or float8"):
         kernels.cache_q8(2, 1, 16, dtype=BF, device="cpu")
     with pytest.raises(ValueError, match="slots"):
-        kernels._ints(torch.zeros(4, dtype=torch.int64), "slots", dev)
+        kernels._check_ints(torch.zeros(4, dtype=torch.int64), "slots", dev)
     assert kernels._cache_args(*kernels.cache_q8(2, 3, 32, 64, dtype=torch.float8_e4m3fn, device="cpu"), dev) == (2, 3, 32, 64, 1)
 
 
