@@ -46,21 +46,24 @@ struct CacheAttnArgs {
   void* out;
   int64_t out_row, out_head;
   float* lse;                 // [q_rows][heads * group] or null
-  int vec;                    // q rows start on 16-byte boundaries
+  int vec, out_vec;           // rows of q and of out start on 16-byte boundaries
+  int rows_from, rows_to;     // the requests whose rows times group lie in between are this launch's
   // parts of cut units: per warp and per CTA a front and a tail, [rows of a tile][dim] sums and their (m, M, l)
   float *part, *cta_part;
   float4 *stat, *cta_stat;
-  int4* desc;                 // [CTAs] rows | last CTA << 8, request, row tile, head of the unit that the CTA begins
+  int4* desc;                 // [CTAs] rows | last CTA << 9, request, row tile, head of the unit that the CTA begins
 };
 
 struct CacheReq {
   int row0, n, len, origin;
 };
 
+// Request r as this launch sees it (n = 0: nothing to do).
 __device__ __forceinline__ CacheReq cache_request(const CacheAttnArgs& a, int r) {
   CacheReq q;
   q.row0 = min(max(a.row_start[r], 0), a.q_rows);
   q.n = max(0, min(a.row_start[r + 1], a.q_rows) - q.row0);
+  if (q.n * a.group < a.rows_from || q.n * a.group > a.rows_to) q.n = 0;  // another launch's
   q.len = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[r], 0)), static_cast<int64_t>(a.width) * a.block));
   q.origin = a.origin ? max(a.origin[r], 0) : 0;
   return q;
@@ -790,7 +793,7 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
       }
     }
     if (s >= 0 && !done && tid == 0)  // cut at the CTA's end: its owner's descriptor
-      a.desc[blockIdx.x] = make_int4(rows | ends[s].last << 8, ends[s].r, ends[s].t, ends[s].h);
+      a.desc[blockIdx.x] = make_int4(rows | ends[s].last << 9, ends[s].r, ends[s].t, ends[s].h);
     if (s >= 0 && !done) return;      // the last chain
   }
   if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -813,7 +816,7 @@ __global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const Cach
   const int base = blockIdx.x * kQmWarps;
   int4 mine = make_int4(0, 0, 0, 0);  // lane i of every warp holds owner base + i
   if (lane < kQmWarps && base + lane < ctas) mine = a.desc[base + lane];
-  const int my_parts = (mine.x >> 8) - (base + lane) + 1, my_rows = mine.x & 255;
+  const int my_parts = (mine.x >> 9) - (base + lane) + 1, my_rows = mine.x & 511;
   for (int row = blockIdx.y; row < kRows; row += gridDim.y) {
     const uint32_t alone = __ballot_sync(~0u, row < my_rows && my_parts <= kQmAlone);
     uint32_t many = __ballot_sync(~0u, row < my_rows && my_parts > kQmAlone);

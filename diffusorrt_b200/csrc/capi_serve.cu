@@ -8,6 +8,7 @@
 #include <cstring>
 
 #include "attention_q8.cuh"
+#include "attention_q8_tiles.cuh"
 #include "capi_common.h"
 #include "kvcache.cuh"
 #include "logprobs.cuh"
@@ -195,50 +196,83 @@ extern "C" int drt_cache_read(const int32_t* slots, int32_t rows, const void* k_
 
 // ======================================================================= attention over the cache
 namespace {
+constexpr int kFewRows = 16;    // a row tile of the kernel for few rows
+constexpr int kManyRows = 48;   // average rows from which small requests ride along in the kernel for many
+
 constexpr size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// Lays a call's scratch out from `base` and returns its size: the cut units' parts of every warp and CTA.
-size_t attend_scratch(int sms, int dim, uint8_t* base, CacheAttnArgs* a) {
+// Lays a call's scratch out from `base` and returns its size: the cut units' parts of every warp and CTA, for the
+// launch over few rows (`few`) and the one over many.
+size_t attend_scratch(int sms, int dim, uint8_t* base, CacheAttnArgs* few, CacheAttnArgs* many) {
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t* p = base + at;
     at += up256(bytes);
     return p;
   };
-  const size_t warp_rows = static_cast<size_t>(sms) * kQrMaxParts, cta_rows = static_cast<size_t>(sms) * 2 * kQrMaxRows;
-  a->part = reinterpret_cast<float*>(take(warp_rows * dim * 4));
-  a->stat = reinterpret_cast<float4*>(take(warp_rows * 16));
-  a->cta_part = reinterpret_cast<float*>(take(cta_rows * dim * 4));
-  a->cta_stat = reinterpret_cast<float4*>(take(cta_rows * 16));
-  a->desc = reinterpret_cast<int4*>(take(static_cast<size_t>(sms) * 16));
+  const size_t warp_rows = static_cast<size_t>(sms) * kQrMaxParts;
+  few->part = reinterpret_cast<float*>(take(warp_rows * dim * 4));
+  few->stat = reinterpret_cast<float4*>(take(warp_rows * 16));
+  auto ctas = [&](CacheAttnArgs* a, int tile_rows) {
+    const size_t rows = static_cast<size_t>(sms) * 2 * tile_rows;
+    a->cta_part = reinterpret_cast<float*>(take(rows * dim * 4));
+    a->cta_stat = reinterpret_cast<float4*>(take(rows * 16));
+    a->desc = reinterpret_cast<int4*>(take(static_cast<size_t>(sms) * 16));
+  };
+  ctas(few, kQrMaxRows);
+  ctas(many, kQtRows);
   return at;
 }
 
+template <typename T, int kDim, int kRows>
+cudaError_t run_merge(const CacheAttnArgs& a, int grid, int64_t rows, cudaStream_t st) {
+  return launch(cache_attn_merge_kernel<T, kDim, kRows>,
+                dim3((grid + kQmWarps - 1) / kQmWarps, static_cast<unsigned>(std::min<int64_t>(rows, kRows))), dim3(kQmThreads), 0,
+                st, true, a, grid);
+}
+
+// rows: the most rows of one kv head's queries in a request; tiles: an upper bound on the key tiles of all units;
+// deep: a unit's, 1 if nothing can be cut.
 template <typename T, int kDim, int kCode, int kNT>
-cudaError_t run_rows_nt(const CacheAttnArgs& a, int device, int64_t tiles, int sms, int merge_rows, cudaStream_t st) {
+cudaError_t run_rows_nt(const CacheAttnArgs& a, int device, int sms, int64_t rows, int64_t tiles, int64_t deep, cudaStream_t st) {
   using Cfg = QrCfg<kDim, kNT>;
   const int grid = static_cast<int>(std::min<int64_t>(sms, tiles));
   cudaError_t e = allow_smem<cache_attn_rows_kernel<T, kDim, kCode, kNT>>(device, Cfg::kSmem);
   if (e == cudaSuccess)
     e = launch(cache_attn_rows_kernel<T, kDim, kCode, kNT>, dim3(grid), dim3(Cfg::kThreads), Cfg::kSmem, st, false, a);
-  if (e != cudaSuccess || merge_rows == 0) return e;
-  return launch(cache_attn_merge_kernel<T, kDim, Cfg::kRows>,
-                dim3((grid + kQmWarps - 1) / kQmWarps, std::min(merge_rows, Cfg::kRows)), dim3(kQmThreads), 0, st, true, a, grid);
+  if (e == cudaSuccess && deep > 1) e = run_merge<T, kDim, Cfg::kRows>(a, grid, rows, st);
+  return e;
 }
 
-// Eight rows to a tile where the caller's bound says that a kv head's rows fit, else sixteen.
 template <typename T, int kDim, int kCode>
-cudaError_t run_rows(const CacheAttnArgs& a, int device, int64_t rows, int64_t tiles, int sms, int merge_rows, cudaStream_t st) {
-  return rows <= 8 ? run_rows_nt<T, kDim, kCode, 1>(a, device, tiles, sms, merge_rows, st)
-                   : run_rows_nt<T, kDim, kCode, 2>(a, device, tiles, sms, merge_rows, st);
+cudaError_t run_attend(const CacheAttnArgs& few, const CacheAttnArgs& many, int device, int sms, int64_t rows, int64_t width,
+                       cudaStream_t st) {
+  const int64_t total = static_cast<int64_t>(few.q_rows) * few.group;
+  auto tiles = [&](int tile_rows, int64_t deep) { return (total / tile_rows + few.requests) * few.heads * deep; };
+  cudaError_t e = cudaSuccess;
+  if (few.rows_from <= few.rows_to) {
+    // eight rows to a tile where the caller's bound says that a kv head's rows fit, else sixteen
+    const int64_t deep = (width + kQrTile - 1) / kQrTile;
+    e = rows <= 8 ? run_rows_nt<T, kDim, kCode, 1>(few, device, sms, rows, tiles(8, deep), deep, st)
+                  : run_rows_nt<T, kDim, kCode, 2>(few, device, sms, rows, tiles(16, deep), deep, st);
+  }
+  if (e == cudaSuccess && many.rows_from <= many.rows_to) {
+    const int64_t deep = (width + kQtKeys - 1) / kQtKeys;
+    const int grid = static_cast<int>(std::min<int64_t>(sms, tiles(kQtRows, deep)));
+    e = allow_smem<cache_attn_tiles_kernel<T, kDim, kCode>>(device, QtCfg<kDim>::kSmem);
+    if (e == cudaSuccess)
+      e = launch(cache_attn_tiles_kernel<T, kDim, kCode>, dim3(grid), dim3(kQtThreads), QtCfg<kDim>::kSmem, st, false, many);
+    if (e == cudaSuccess && deep > 1) e = run_merge<T, kDim, kQtRows>(many, grid, rows, st);
+  }
+  return e;
 }
 }  // namespace
 
 extern "C" size_t drt_cache_attend_scratch_bytes(int32_t dim) {
   int device = 0;
   const int sms = current_sms(&device);
-  CacheAttnArgs a;
-  return attend_scratch(sms > 0 ? sms : 148, dim, nullptr, &a);
+  CacheAttnArgs a, b;
+  return attend_scratch(sms > 0 ? sms : 148, dim, nullptr, &a, &b);
 }
 
 extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
@@ -287,17 +321,24 @@ extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
   a.out_head = p->out_head;
   a.lse = p->lse;
   a.vec = aligned16(p->q) && (p->q_row | p->q_head) % 8 == 0;
-  attend_scratch(sms, p->dim, static_cast<uint8_t*>(p->scratch), &a);
+  a.out_vec = aligned16(p->out) && (p->out_row | p->out_head) % 8 == 0;
+  // Rows of one kv head in a request: up to kFewRows go to the kernel for few, the rest to the one for many. One launch
+  // where the caller's bound or the average says that the other would find (nearly) nothing; either serves any count.
+  CacheAttnArgs b = a;
+  attend_scratch(sms, p->dim, static_cast<uint8_t*>(p->scratch), &a, &b);
   const int max_rows = p->max_rows > 0 ? std::min(p->max_rows, p->q_rows) : p->q_rows;
-  // A unit's key tiles at most: with one there is nothing to cut and nothing to join.
-  const int64_t deep = (static_cast<int64_t>(p->width) * p->block + kQrTile - 1) / kQrTile;
-  const int64_t units = (static_cast<int64_t>(p->q_rows) * a.group / 8 + p->requests) * a.heads;
   const int64_t rows = static_cast<int64_t>(max_rows) * a.group;
-  const int merge_rows = deep > 1 ? static_cast<int>(std::min<int64_t>(kQrMaxRows, rows)) : 0;
+  const int64_t average = static_cast<int64_t>(p->q_rows) * a.group / p->requests;
+  const bool only_few = rows <= kFewRows, only_many = !only_few && average >= kManyRows;
+  a.rows_from = only_many ? 1 : 0;
+  a.rows_to = only_many ? 0 : only_few ? INT32_MAX : kFewRows;
+  b.rows_from = only_few ? 1 : only_many ? 0 : kFewRows + 1;
+  b.rows_to = only_few ? 0 : INT32_MAX;
   const int dim = p->dim, code = p->code;
+  const int64_t width = static_cast<int64_t>(p->width) * p->block;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CK(p->dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_rows, __nv_bfloat16, a, device, rows, units * deep, sms, merge_rows, st)
-                               : DRT_DISPATCH_DIM_CODE(run_rows, __half, a, device, rows, units * deep, sms, merge_rows, st));
+  CK(p->dtype == DRT_TYPE_BF16 ? DRT_DISPATCH_DIM_CODE(run_attend, __nv_bfloat16, a, b, device, sms, rows, width, st)
+                               : DRT_DISPATCH_DIM_CODE(run_attend, __half, a, b, device, sms, rows, width, st));
   return DRT_OK;
 }
 

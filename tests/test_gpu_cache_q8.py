@@ -416,6 +416,15 @@ def test_attend_many_rows(kernels, mask_block, dim, code, typ):
     check_attend(kernels, attend_case(16, requests, 6, 2, dim, 32, code, typ, pad=4), mask_block)
 
 
+@pytest.mark.parametrize("dim,code,typ,heads,kv_heads", [(128, E4, BF, 4, 2), (64, I8, HF, 3, 1), (128, I8, HF, 2, 2)])
+def test_attend_many_rows_over_long_prefixes(kernels, dim, code, typ, heads, kv_heads):
+    """Units of many key tiles, cut between shares and joined; one and two row tiles; rows that the tile does not fill."""
+    requests = [(129, 2500), (40, 3001), (0, 9), (7, 1100), (260, 260), (64, 640)]
+    case = attend_case(22, requests, heads, kv_heads, dim, 128, code, typ, pad=2)
+    for mask_block in (1, 32):
+        check_attend(kernels, case, mask_block, origin=[100, 0, 0, 2000, 64, 7])
+
+
 def test_attend_bound_on_rows_changes_nothing_but_speed(kernels):
     """max_rows is a hint: requests with more rows are served all the same."""
     case = attend_case(17, [(40, 100), (3, 80)], 8, 2, 128, 32, I8, BF)
