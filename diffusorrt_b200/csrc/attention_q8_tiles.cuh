@@ -4,8 +4,8 @@
 //
 // With this many rows the work is products, so it belongs on tcgen05 (kind::f16, f32 accumulators in TMEM), which
 // wants the codes as f16 in shared memory. The roles, one CTA per SM:
-//   loader   (1 warp)  bulk copies of the codes, 2 KB per 16-token group, K and V tiles in turn; the blocks' scales
-//   expander (4 warps) codes -> f16 in the 128-byte swizzled K-major layout: K [keys x dims], V^T [dims x keys]
+//   loader   (1 warp of the expander)  bulk copies of the codes, 2 KB per 16-token group, K and V in turn; the scales
+//   expander (3 warps) codes -> f16 in the 128-byte swizzled K-major layout: K [keys x dims], V^T [dims x keys]
 //   issuer   (1 warp)  S_X = Q_X K^T, O_X += W_X V for X = A, B; the two tiles share the expanded codes, and one
 //                      tile's products run while the other's softmax does
 //   softmax  (8 warps) a thread per row: S from TMEM, W = f16 weights back to TMEM over S (the A operand of the second
@@ -22,7 +22,8 @@ namespace drt {
 constexpr int kQtRows = 256;
 constexpr int kQtKeys = 128;
 constexpr int kQtGroups = kQtKeys / 16;
-constexpr int kQtThreads = 448;
+constexpr int kQtThreads = 384;     // 12 warps, so that the softmax has 168 registers a thread
+constexpr int kQtExpand = 96;       // threads of the expander
 constexpr int kQtMeta = 8;          // key tiles whose scales are kept: the loader is at most five ahead of the softmax
 
 template <int kDim>
@@ -35,9 +36,11 @@ struct QtCfg {
   static constexpr size_t kSmem = 1024 + kEnd;     // tiles on 1024-byte boundaries
 };
 
-struct QtMeta {
-  float c[kQtGroups], lv[kQtGroups];  // ks scale log2(e); log2 vs
-  int live[kQtGroups];                // tokens of the group that the unit sees; 0 also for a missing block
+struct __align__(16) QtMeta {
+  float c[kQtGroups], lv[kQtGroups], iv[kQtGroups];  // per group ks scale log2(e), log2 vs, 1 / vs
+  int live[kQtGroups];       // tokens of the group that the unit sees; 0 also for a missing block
+  int full;                  // every group has 16
+  float lv_low, lv_high;     // over the groups
 };
 
 // f16 x f16 -> f32, both K-major.
@@ -62,6 +65,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
 struct QtBars {
   uint64_t raw_full[2], raw_empty[2];   // codes of K, codes of V
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
@@ -82,10 +105,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.raw_full[i], 1);
-      mbar_init(&bar.raw_empty[i], 4);
-      mbar_init(&bar.k_full[i], 4);
+      mbar_init(&bar.raw_empty[i], kQtExpand / 32);
+      mbar_init(&bar.k_full[i], kQtExpand / 32);
       mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], 4);
+      mbar_init(&bar.v_full[i], kQtExpand / 32);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.q_full[i], 4);
       mbar_init(&bar.s_full[i], 1);
@@ -96,7 +119,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
     bar.failed = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 11) {
     tmem_alloc(&bar.tmem, 512);
     tmem_relinquish();
   }
@@ -156,136 +179,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
   auto segment = [&] { return static_cast<int>(min(static_cast<int64_t>(cur.L - kt), x_end - x)); };
   const uint32_t smem_at = smem_u32(smem);
 
-  if (warp == 13) {
-    // ------------------------------------------------------------ loader
-    const int block_shift = 31 - __clz(a.block);
-    uint32_t n = 0;          // key tiles loaded
-    bool ok = true;
-    while (x < x_end && ok) {
-      const int tiles = segment();
-      // lane = tile * 8 + group of four tiles; the next four's table entries are read ahead
-      auto entry = [&](int tile0) {
-        const int tok = (kt + tile0 + (lane >> 3)) * kQtKeys + (lane & 7) * 16;
-        return tile0 + (lane >> 3) < tiles && tok < cur.lim ? a.tables[cur.r * a.ld_tables + (tok >> block_shift)] : -1;
-      };
-      int id_next = entry(0), id = -1;
-      float ks = 0.0f, vs = 0.0f;
-      for (int j = 0; j < tiles && ok; ++j, ++n) {
-        if ((j & 3) == 0) {
-          id = id_next;
-          id_next = entry(j + 4);
-          if (id >= a.blocks) id = -1;
-          ks = vs = 0.0f;
-          if (id >= 0) {
-            ks = a.k_scale[static_cast<int64_t>(id) * a.heads + cur.h];
-            vs = a.v_scale[static_cast<int64_t>(id) * a.heads + cur.h];
-          }
-        }
-        const int pg = __shfl_sync(~0u, id, (j & 3) * 8 + (lane & 7));
-        const float k = __shfl_sync(~0u, ks, (j & 3) * 8 + (lane & 7)), v = __shfl_sync(~0u, vs, (j & 3) * 8 + (lane & 7));
-        const int tok = (kt + j) * kQtKeys + (lane & 7) * 16;
-        const uint32_t have = __ballot_sync(~0u, pg >= 0) & 0xffu;
-        const int64_t src = (((static_cast<int64_t>(pg) * a.heads + cur.h) << block_shift) + (tok & (a.block - 1))) * kDim;
-#pragma unroll
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          ok = __all_sync(~0u, wait(&bar.raw_empty[kv], (n & 1) ^ 1));
-          if (!ok) break;
-          if (kv == 0) {
-            QtMeta& m = metas[n % kQtMeta];
-            if (lane < 8) {
-              m.c[lane] = k * a.scale_log2;
-              m.lv[lane] = pg >= 0 ? log2f(v) : -INFINITY;
-              m.live[lane] = pg >= 0 ? min(16, cur.lim - tok) : 0;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.meta_full[n % kQtMeta]);
-          }
-          if (lane == 0) mbar_expect_tx(&bar.raw_full[kv], __popc(have) * 16 * kDim);
-          __syncwarp();
-          if (lane < 8 && pg >= 0)
-            bulk_load(smem_at + Cfg::kCodes + kv * Cfg::kRaw + lane * 16 * kDim, (kv ? a.v_cache : a.k_cache) + src, 16 * kDim,
-                      &bar.raw_full[kv]);
-        }
-        ok = ok && !*failed;
-      }
-      advance(tiles);
-    }
-    if (!ok && n > 0) {  // copies under way land before the shared memory is given up
-      mbar_wait(&bar.raw_full[0], (n - 1) & 1);
-      mbar_wait(&bar.raw_full[1], (n - 1) & 1);
-    }
-  } else if (warp >= 8 && warp < 12) {
-    // ------------------------------------------------------------ expander
-    const int t = tid - 256;
-    uint32_t n = 0;
-    bool ok = true;
-    while (x < x_end && ok) {
-      const int tiles = segment();
-      for (int j = 0; j < tiles && ok; ++j, ++n) {
-        const int st = n % Cfg::kStages;
-        const uint32_t round = n / Cfg::kStages;
-        // K: a token's 16 dimensions to two 16-byte chunks of its row
-        ok = wait(&bar.raw_full[0], n & 1) && wait(&bar.k_empty[st], (round & 1) ^ 1);
-        if (!(ok = __all_sync(~0u, ok))) break;
-        uint8_t* dst = smem + Cfg::kK + st * Cfg::kTile;
-        const uint8_t* raw = smem + Cfg::kCodes;
-#pragma unroll 4
-        for (int i = t; i < Cfg::kRaw / 16; i += 128) {
-          const uint4 u = *reinterpret_cast<const uint4*>(raw + i * 16);
-          const int tok = i / (kDim / 16), d = (i % (kDim / 16)) * 16;
-          uint4 lo, hi;
-          codes_to_f16<kCode>(u.x, lo.x, lo.y);
-          codes_to_f16<kCode>(u.y, lo.z, lo.w);
-          codes_to_f16<kCode>(u.z, hi.x, hi.y);
-          codes_to_f16<kCode>(u.w, hi.z, hi.w);
-          const bool odd = d >= 64;  // lanes of the second atom write their chunks in the other order: other banks
-          *reinterpret_cast<uint4*>(dst + sw128_offset(tok, d + (odd ? 8 : 0), kQtKeys)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + sw128_offset(tok, d + (odd ? 0 : 8), kQtKeys)) = odd ? lo : hi;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bar.k_full[st]);
-          mbar_arrive(&bar.raw_empty[0]);
-        }
-        // V: a dimension's 16 tokens to two chunks of its row of V^T; tokens nobody sees become 0, since 0 times
-        // whatever they hold need not be 0
-        ok = wait(&bar.raw_full[1], n & 1) && wait(&bar.v_empty[st], (round & 1) ^ 1);
-        if (!(ok = __all_sync(~0u, ok))) break;
-        dst = smem + Cfg::kV + st * Cfg::kTile;
-        raw = smem + Cfg::kCodes + Cfg::kRaw;
-        const QtMeta& m = metas[n % kQtMeta];
-#pragma unroll 4
-        for (int i = t; i < Cfg::kRaw / 16; i += 128) {
-          uint4 u = *reinterpret_cast<const uint4*>(raw + i * 16);
-          const int grp = i / kDim, d = i % kDim;
-          const int live = m.live[grp];
-          if (live < 16) {
-            auto keep = [&](int w) {
-              const int c = min(4, max(0, live - 4 * w));
-              return c >= 4 ? ~0u : (1u << (8 * c)) - 1u;
-            };
-            u = make_uint4(u.x & keep(0), u.y & keep(1), u.z & keep(2), u.w & keep(3));
-          }
-          uint4 lo, hi;
-          codes_to_f16<kCode>(u.x, lo.x, lo.y);
-          codes_to_f16<kCode>(u.y, lo.z, lo.w);
-          codes_to_f16<kCode>(u.z, hi.x, hi.y);
-          codes_to_f16<kCode>(u.w, hi.z, hi.w);
-          *reinterpret_cast<uint4*>(dst + sw128_offset(d, grp * 16, kDim)) = lo;
-          *reinterpret_cast<uint4*>(dst + sw128_offset(d, grp * 16 + 8, kDim)) = hi;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bar.v_full[st]);
-          mbar_arrive(&bar.raw_empty[1]);
-        }
-        ok = !*failed;
-      }
-      advance(tiles);
-    }
-  } else if (warp == 12) {
+  if (warp == 11) {
     // ------------------------------------------------------------ issuer
     const uint32_t idesc_s = idesc_f16_f32(128, kQtKeys), idesc_o = idesc_f16_f32(128, kDim);
     uint32_t n = 0;                   // key tiles whose second product is issued
@@ -345,6 +239,158 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
         ok = __all_sync(~0u, ok && !*failed);
       }
       advance(tiles);
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ expander; its first warp is the loader too
+    const int ew = warp - 8;
+    // 32 16-byte reads at a time, dealt to the three warps
+    constexpr int kParts = Cfg::kRaw / 512, kTurns = (kParts + kQtExpand / 32 - 1) / (kQtExpand / 32);
+    auto put2 = [](uint8_t* dst, uint32_t at0, uint32_t at1, const uint4& u) {
+      uint4 lo, hi;
+      codes_to_f16<kCode>(u.x, lo.x, lo.y);
+      codes_to_f16<kCode>(u.y, lo.z, lo.w);
+      codes_to_f16<kCode>(u.z, hi.x, hi.y);
+      codes_to_f16<kCode>(u.w, hi.z, hi.w);
+      *reinterpret_cast<uint4*>(dst + at0) = lo;
+      *reinterpret_cast<uint4*>(dst + at1) = hi;
+    };
+    auto expand_k = [&](const uint8_t* raw, uint8_t* dst) {  // a token's 16 dimensions
+      const int sub = lane / (kDim / 16), d = (lane % (kDim / 16)) * 16;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int part = ew + i * (kQtExpand / 32);
+        if (part < kParts) {
+          const int tok = part * (512 / kDim) + sub;
+          put2(dst, sw128_offset(tok, d, kQtKeys), sw128_offset(tok, d + 8, kQtKeys),
+               *reinterpret_cast<const uint4*>(raw + part * 512 + lane * 16));
+        }
+      }
+    };
+    auto expand_v = [&](const uint8_t* raw, uint8_t* dst, auto full, const QtMeta& m) {  // a dimension's 16 tokens
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int part = ew + i * (kQtExpand / 32);
+        if (part < kParts) {
+          const int grp = part / (kDim / 32), d = part % (kDim / 32) * 32 + lane;
+          uint4 u = *reinterpret_cast<const uint4*>(raw + part * 512 + lane * 16);
+          if constexpr (!decltype(full)::value) {
+            const int live = m.live[grp];
+            auto keep = [&](int w) {
+              const int c = min(4, max(0, live - 4 * w));
+              return c >= 4 ? ~0u : (1u << (8 * c)) - 1u;
+            };
+            u = make_uint4(u.x & keep(0), u.y & keep(1), u.z & keep(2), u.w & keep(3));
+          }
+          put2(dst, sw128_offset(d, grp * 16, kDim), sw128_offset(d, grp * 16 + 8, kDim), u);
+        }
+      }
+    };
+    const int block_shift = 31 - __clz(a.block);
+    uint32_t n = 0;          // key tiles expanded
+    bool ok = true;
+    while (x < x_end && ok) {
+      const int tiles = segment();
+      // table entries and scales of four key tiles at a time: lane = tile * 8 + group; the next four's are read ahead
+      auto entry = [&](int tile0) {
+        const int tok = (kt + tile0 + (lane >> 3)) * kQtKeys + (lane & 7) * 16;
+        return tile0 + (lane >> 3) < tiles && tok < cur.lim ? a.tables[cur.r * a.ld_tables + (tok >> block_shift)] : -1;
+      };
+      const uint32_t n0 = n;
+      int id = -1, id_next = -1;
+      float ks = 0.0f, vs = 0.0f;
+      if (warp == 8) id_next = entry(0);
+      // Asks for the codes of key tile j (K, or V) once their place is free, and tells the softmax its scales.
+      auto load = [&](int j, bool is_v) -> bool {
+        if (!is_v && (j & 3) == 0) {
+          id = id_next < a.blocks ? id_next : -1;
+          id_next = entry(j + 4);
+          ks = vs = 0.0f;
+          if (id >= 0) {
+            ks = a.k_scale[static_cast<int64_t>(id) * a.heads + cur.h];
+            vs = a.v_scale[static_cast<int64_t>(id) * a.heads + cur.h];
+          }
+        }
+        const uint32_t nj = n0 + j;
+        const int from = (j & 3) * 8 + (lane & 7);
+        const int pg = __shfl_sync(~0u, id, from);
+        const int tok = (kt + j) * kQtKeys + (lane & 7) * 16;
+        if (!__all_sync(~0u, wait(&bar.raw_empty[is_v], (nj & 1) ^ 1))) return false;
+        if (!is_v) {
+          QtMeta& m = metas[nj % kQtMeta];
+          const float k = __shfl_sync(~0u, ks, from), v = __shfl_sync(~0u, vs, from);
+          const float lv = pg >= 0 ? log2f(v) : -INFINITY;
+          const int live = pg >= 0 ? min(16, cur.lim - tok) : 0;
+          float low = lv, high = lv;
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) {
+            low = fminf(low, __shfl_xor_sync(~0u, low, d));
+            high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
+          }
+          const uint32_t full = __ballot_sync(~0u, live == 16) & 0xffu;
+          if (lane < 8) {
+            m.c[lane] = k * a.scale_log2;
+            m.lv[lane] = lv;
+            m.iv[lane] = 1.0f / v;
+            m.live[lane] = live;
+          }
+          if (lane == 0) {
+            m.full = full == 0xffu;
+            m.lv_low = low;
+            m.lv_high = high;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.meta_full[nj % kQtMeta]);
+        }
+        const uint32_t have = __ballot_sync(~0u, pg >= 0) & 0xffu;
+        if (lane == 0) mbar_expect_tx(&bar.raw_full[is_v], __popc(have) * 16 * kDim);
+        __syncwarp();
+        if (lane < 8 && pg >= 0)
+          bulk_load(smem_at + Cfg::kCodes + is_v * Cfg::kRaw + lane * 16 * kDim,
+                    (is_v ? a.v_cache : a.k_cache) +
+                        (((static_cast<int64_t>(pg) * a.heads + cur.h) << block_shift) + (tok & (a.block - 1))) * kDim,
+                    16 * kDim, &bar.raw_full[is_v]);
+        return true;
+      };
+      if (warp == 8) ok = load(0, false) && load(0, true);
+      for (int j = 0; j < tiles && ok; ++j, ++n) {
+        const int st = n % Cfg::kStages;
+        const uint32_t round = n / Cfg::kStages;
+        // K: a token's 16 dimensions to two 16-byte chunks of its row
+        ok = wait(&bar.raw_full[0], n & 1) && wait(&bar.k_empty[st], (round & 1) ^ 1);
+        if (!(ok = __all_sync(~0u, ok))) break;
+        uint8_t* dst = smem + Cfg::kK + st * Cfg::kTile;
+        const uint8_t* raw = smem + Cfg::kCodes;
+        expand_k(raw, dst);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.k_full[st]);
+          mbar_arrive(&bar.raw_empty[0]);
+        }
+        if (warp == 8 && j + 1 < tiles) ok = load(j + 1, false);
+        // V: a dimension's 16 tokens to two chunks of its row of V^T; tokens nobody sees become 0, since 0 times
+        // whatever they hold need not be 0
+        ok = ok && wait(&bar.raw_full[1], n & 1) && wait(&bar.v_empty[st], (round & 1) ^ 1);
+        if (!(ok = __all_sync(~0u, ok))) break;
+        dst = smem + Cfg::kV + st * Cfg::kTile;
+        raw = smem + Cfg::kCodes + Cfg::kRaw;
+        const QtMeta& m = metas[n % kQtMeta];
+        if (m.full) expand_v(raw, dst, std::true_type(), m);
+        else expand_v(raw, dst, std::false_type(), m);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.v_full[st]);
+          mbar_arrive(&bar.raw_empty[1]);
+        }
+        if (warp == 8 && j + 1 < tiles) ok = load(j + 1, true);
+        ok = __all_sync(~0u, ok && !*failed);
+      }
+      advance(tiles);
+    }
+    if (!ok && warp == 8) {  // copies under way land before the shared memory is given up (bounded waits)
+      mbar_wait(&bar.raw_full[0], n & 1);
+      mbar_wait(&bar.raw_full[1], n & 1);
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -419,33 +465,52 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
         tc_fence_after();
         const QtMeta& meta = metas[n % kQtMeta];
         const int key0 = (kt + j) * kQtKeys;
-        bool whole = key0 + kQtKeys <= lim;
+        const bool edge = __any_sync(~0u, !meta.full || key0 + kQtKeys > lim);
+        // ---- the tile's maxima, of the scores and of the scores with log2 vs
+        float v[64], t = -INFINITY, u = -INFINITY;
+        if (!edge) {
+          // the later half first, so that the earlier one is in registers when the weights are written over its columns
+          float c[kQtGroups], lv[kQtGroups];
 #pragma unroll
-        for (int g = 0; g < kQtGroups; ++g) whole = whole && meta.live[g] == 16;
-        const bool edge = __any_sync(~0u, !whole);
-        // ---- the tile's maxima: of the scores, and of the scores with log2 vs
-        float t = -INFINITY, u = -INFINITY;
+          for (int g = 0; g < kQtGroups; ++g) {
+            c[g] = meta.c[g] * f;
+            lv[g] = meta.lv[g];
+          }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32(s_at + c * 32, v);
+          for (int half = 1; half >= 0; --half) {
+            tmem_ld32x2(s_at + half * 64, v);
+            float g_max[4];
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int g = c * 2 + hf;
-            float mx = -INFINITY;
-            if (edge) {
-              const int see = min(meta.live[g], lim - key0 - g * 16);
+            for (int g = 0; g < 4; ++g) {
+              float q[4];
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (e < see) mx = fmaxf(mx, v[hf * 16 + e]);
-              mx = see > 0 ? mx * (meta.c[g] * f) : -INFINITY;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) mx = fmaxf(mx, v[hf * 16 + e]);
-              mx *= meta.c[g] * f;
+              for (int e = 0; e < 4; ++e)
+                q[e] = fmaxf(fmaxf(v[g * 16 + e], v[g * 16 + 4 + e]), fmaxf(v[g * 16 + 8 + e], v[g * 16 + 12 + e]));
+              g_max[g] = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
             }
-            t = fmaxf(t, mx);
-            if (mx > -INFINITY) u = fmaxf(u, mx + meta.lv[g]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float s = g_max[g] * c[half * 4 + g];
+              t = fmaxf(t, s);
+              u = fmaxf(u, s + lv[half * 4 + g]);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld32(s_at + c * 32, v);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const int g = c * 2 + hf, see = min(meta.live[g], lim - key0 - g * 16);
+              float mx = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) mx = e < see ? fmaxf(mx, v[hf * 16 + e]) : mx;
+              if (mx > -INFINITY) {  // else all hidden (a scale of 0 is legal, and 0 * -inf is not a score)
+                mx *= meta.c[g] * f;
+                t = fmaxf(t, mx);
+                u = fmaxf(u, mx + meta.lv[g]);
+              }
+            }
           }
         }
         // ---- move the references where they are too low
@@ -460,50 +525,81 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
             ok = __all_sync(~0u, wait(&bar.pv_done[X], mine - 1));
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < kDim / 32; ++c) {
-              float v[32];
-              tmem_ld32(o_at + c * 32, v);
+#pragma unroll 1
+            for (int c = 0; c < kDim; c += 32) {
+              float o[32];
+              tmem_ld32(o_at + c, o);
               uint32_t w[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(v[e] * kM);
-              tmem_st16(o_at + c * 32, w);
-              tmem_st16(o_at + c * 32 + 16, w + 16);
+              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * kM);
+              tmem_st16(o_at + c, w);
+              tmem_st16(o_at + c + 16, w + 16);
             }
-            tmem_wait_st();
           }
         }
         const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
-        // ---- weights, over S: 32 scores become 16 columns that have been read
+        // ---- weights 2^(s - z) f_g, f_g = vs 2^(z - Z), over S's columns that have been read. Where every f_g lies within
+        // 2^+-60 it joins the exponent, and a group's sum of weights over f_g is that of its probabilities.
+        const bool near = meta.lv_low + (z - Z) >= -60.0f && meta.lv_high + (z - Z) <= 60.0f;
+        const bool fast = __all_sync(~0u, near) && !edge;
+        float p_sum = 0.0f;
+        if (fast) {
+          float c[kQtGroups], off[kQtGroups], iv[kQtGroups];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32(s_at + c * 32, v);
-          uint32_t w[16];
+          for (int g = 0; g < kQtGroups; ++g) {
+            c[g] = meta.c[g] * f;
+            off[g] = meta.lv[g] - Z;
+            iv[g] = meta.iv[g];
+          }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int g = c * 2 + hf;
-            const float k = meta.c[g] * f, wt = qa_ex2(fminf(meta.lv[g] + (z - Z), 120.0f));
-            if (edge) {
-              const int see = min(meta.live[g], lim - key0 - g * 16);
+          for (int half = 0; half < 2; ++half) {
+            if (half == 1) tmem_ld32x2(s_at + 64, v);
+#pragma unroll
+            for (int g2 = 0; g2 < 4; g2 += 2) {
+              uint32_t w[16];
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const int g = g2 + hf, q = half * 4 + g;
+                const float2 kk = make_float2(c[q], c[q]), dd = make_float2(off[q], off[q]);
+                float2 s0 = make_float2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                  float2 y0 = fma2(make_float2(v[g * 16 + e], v[g * 16 + e + 1]), kk, dd);
+                  float2 y1 = fma2(make_float2(v[g * 16 + e + 2], v[g * 16 + e + 3]), kk, dd);
+                  y0 = make_float2(qa_ex2(y0.x), qa_ex2(y0.y));
+                  y1 = make_float2(qa_ex2(y1.x), qa_ex2(y1.y));
+                  s0 = add2(s0, y0);
+                  s1 = add2(s1, y1);
+                  w[hf * 8 + e / 2] = f16_pair(y0.x, y0.y);
+                  w[hf * 8 + e / 2 + 1] = f16_pair(y1.x, y1.y);
+                }
+                s0 = add2(s0, s1);
+                p_sum = __fmaf_rn(s0.x + s0.y, iv[q], p_sum);
+              }
+              tmem_st16(s_at + half * 32 + g2 * 8, w);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld32(s_at + c * 32, v);
+            uint32_t w[16];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const int g = c * 2 + hf, see = edge ? min(meta.live[g], lim - key0 - g * 16) : 16;
+              const float k = meta.c[g] * f, wt = qa_ex2(fminf(meta.lv[g] + (z - Z), 120.0f));
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
                 const float p0 = e < see ? qa_ex2(__fmaf_rn(v[hf * 16 + e], k, -z)) : 0.0f;
                 const float p1 = e + 1 < see ? qa_ex2(__fmaf_rn(v[hf * 16 + e + 1], k, -z)) : 0.0f;
-                l += p0 + p1;
-                w[hf * 8 + e / 2] = f16_pair(p0 * wt, p1 * wt);
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const float p0 = qa_ex2(__fmaf_rn(v[hf * 16 + e], k, -z)), p1 = qa_ex2(__fmaf_rn(v[hf * 16 + e + 1], k, -z));
-                l += p0 + p1;
+                p_sum += p0 + p1;
                 w[hf * 8 + e / 2] = f16_pair(p0 * wt, p1 * wt);
               }
             }
+            tmem_st16(s_at + c * 16, w);
           }
-          tmem_st16(s_at + c * 16, w);
         }
+        l = fast ? __fmaf_rn(p_sum, qa_ex2(Z - z), l) : l + p_sum;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -556,7 +652,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 11) tmem_dealloc(tmem, 512);
   if (tid == 0) a.desc[blockIdx.x] = owner;
 }
 
