@@ -47,13 +47,38 @@ struct __align__(16) QtMeta {
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
-// As umma_bf16 with the A operand in TMEM (lane = row, a 32-bit column = two consecutive k).
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The low word of sdesc_kmajor_sw128's descriptor; the high word is kDescHigh for every tile here.
+__device__ __forceinline__ uint32_t sdesc_low(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// One of the warp's threads, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Step kk (16 of the contracted index) of D (+)= A B^T. The descriptors are given by their low words, which a step only
+// moves by a constant: two 16-byte units within a 128-byte atom, kAtom units from one atom to the next.
+template <int kAtomA, int kAtomB>
+__device__ __forceinline__ void umma_step_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, int kk, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_low + (kk >> 2) * kAtomA + (kk & 3) * 2), "r"(b_low + (kk >> 2) * kAtomB + (kk & 3) * 2), "r"(idesc),
+      "r"(accumulate), "r"(kDescHigh)
+      : "memory");
+}
+// The same with the A operand in TMEM (lane = row, a 32-bit column = two consecutive k).
+template <int kAtomB>
+__device__ __forceinline__ void umma_step_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, int kk, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem + kk * 8), "r"(b_low + (kk >> 2) * kAtomB + (kk & 3) * 2), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -185,14 +210,13 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
     uint32_t n = 0;                   // key tiles whose second product is issued
     uint32_t units[2] = {0, 0}, done[2] = {0, 0};
     bool ok = true;
+    const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+    const uint32_t q_low = sdesc_low(smem_at + Cfg::kQ), k_low = sdesc_low(smem_at + Cfg::kK), v_low = sdesc_low(smem_at + Cfg::kV);
     auto issue_s = [&](int X, uint32_t tile) {  // S_X of key tile `tile` (a running number)
-      if (lane == 0) {
-        const uint32_t q = smem_at + Cfg::kQ + X * Cfg::kTile, k = smem_at + Cfg::kK + (tile % Cfg::kStages) * Cfg::kTile;
+      const uint32_t ql = q_low + X * (Cfg::kTile / 16), kl = k_low + (tile % Cfg::kStages) * (Cfg::kTile / 16);
+      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kDim / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-          umma_bf16(tmem + X * 128, sdesc_kmajor_sw128(q + off), sdesc_kmajor_sw128(k + off), idesc_s, kk != 0);
-        }
+        for (int kk = 0; kk < kDim / 16; ++kk) umma_step_ss<1024, 1024>(tm + X * 128, ql, kl, idesc_s, kk, kk != 0);
         umma_commit(&bar.s_full[X]);
       }
       __syncwarp();
@@ -207,7 +231,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
         tc_fence_after();
         issue_s(X, n);
       }
-      if (ok && lane == 0) umma_commit(&bar.k_empty[n % Cfg::kStages]);
+      if (ok && elect_one()) umma_commit(&bar.k_empty[n % Cfg::kStages]);
       for (int j = 0; j < tiles && ok; ++j, ++n) {
         const int st = n % Cfg::kStages;
         ok = wait(&bar.v_full[st], n / Cfg::kStages);
@@ -215,13 +239,11 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
           ok = wait(&bar.w_full[X], done[X]++);
           if (!(ok = __all_sync(~0u, ok))) break;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t v = smem_at + Cfg::kV + st * Cfg::kTile;
+          const uint32_t vl = v_low + st * (Cfg::kTile / 16);
+          if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kQtKeys / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * (kDim * 128) + (kk & 3) * 32;
-              umma_ts(tmem + 256 + X * 128, tmem + X * 128 + kk * 8, sdesc_kmajor_sw128(v + off), idesc_o, j > 0 || kk != 0);
-            }
+            for (int kk = 0; kk < kQtKeys / 16; ++kk)
+              umma_step_ts<kDim * 8>(tm + 256 + X * 128, tm + X * 128, vl, idesc_o, kk, j > 0 || kk != 0);
             umma_commit(&bar.pv_done[X]);
           }
           __syncwarp();
@@ -232,7 +254,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
             issue_s(X, n + 1);
           }
         }
-        if (ok && lane == 0) {
+        if (ok && elect_one()) {
           umma_commit(&bar.v_empty[st]);
           if (j + 1 < tiles) umma_commit(&bar.k_empty[(n + 1) % Cfg::kStages]);
         }
