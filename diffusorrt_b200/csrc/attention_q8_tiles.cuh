@@ -4,8 +4,7 @@
 //
 // With this many rows the work is products, so it belongs on tcgen05 (kind::f16, f32 accumulators in TMEM), which
 // wants the codes as f16 in shared memory. The roles, one CTA per SM:
-//   loader   (1 warp of the expander)  bulk copies of the codes, 2 KB per 16-token group, K and V in turn; the scales
-//   expander (3 warps) codes -> f16 in the 128-byte swizzled K-major layout: K [keys x dims], V^T [dims x keys]
+//   expander (3 warps) bulk copies of the codes, 2 KB per 16-token group, and of the blocks' scales; codes -> f16 in the 128-byte swizzled K-major layout: K [keys x dims], V^T [dims x keys]
 //   issuer   (1 warp)  S_X = Q_X K^T, O_X += W_X V for X = A, B; the two tiles share the expanded codes, and one
 //                      tile's products run while the other's softmax does
 //   softmax  (8 warps) a thread per row: S from TMEM, W = f16 weights back to TMEM over S (the A operand of the second
@@ -24,7 +23,9 @@ constexpr int kQtKeys = 128;
 constexpr int kQtGroups = kQtKeys / 16;
 constexpr int kQtThreads = 384;     // 12 warps, so that the softmax has 168 registers a thread
 constexpr int kQtExpand = 96;       // threads of the expander
-constexpr int kQtMeta = 8;          // key tiles whose scales are kept: the loader is at most five ahead of the softmax
+// Key tiles whose scales are kept. They are written four at a time, tiles j to j + 3 once K's tile j - 1 is expanded; that
+// waited for the first product of tile j - 3, so the softmax is done with tile j - 4: seven tiles are in use at most.
+constexpr int kQtMeta = 8;
 
 template <int kDim>
 struct QtCfg {
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
       advance(tiles);
     }
   } else if (warp >= 8) {
-    // ------------------------------------------------------------ expander; its first warp is the loader too
+    // ------------------------------------------------------------ expander
     const int ew = warp - 8;
     // 32 16-byte reads at a time, dealt to the three warps
     constexpr int kParts = Cfg::kRaw / 512, kTurns = (kParts + kQtExpand / 32 - 1) / (kQtExpand / 32);
@@ -312,68 +313,62 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
     bool ok = true;
     while (x < x_end && ok) {
       const int tiles = segment();
-      // table entries and scales of four key tiles at a time: lane = tile * 8 + group; the next four's are read ahead
+      // The first warp asks for K's codes and gives the softmax its scales, the second asks for V's. Table entries of four
+      // key tiles at a time, lane = tile * 8 + group, and the next four's on their way.
       auto entry = [&](int tile0) {
         const int tok = (kt + tile0 + (lane >> 3)) * kQtKeys + (lane & 7) * 16;
         return tile0 + (lane >> 3) < tiles && tok < cur.lim ? a.tables[cur.r * a.ld_tables + (tok >> block_shift)] : -1;
       };
       const uint32_t n0 = n;
-      int id = -1, id_next = -1;
-      float ks = 0.0f, vs = 0.0f;
-      if (warp == 8) id_next = entry(0);
-      // Asks for the codes of key tile j (K, or V) once their place is free, and tells the softmax its scales.
-      auto load = [&](int j, bool is_v) -> bool {
-        if (!is_v && (j & 3) == 0) {
+      int id = -1, id_next = ew < 2 ? entry(0) : -1;
+      auto load = [&](int j, int is_v) -> bool {
+        if ((j & 3) == 0) {
           id = id_next < a.blocks ? id_next : -1;
           id_next = entry(j + 4);
-          ks = vs = 0.0f;
-          if (id >= 0) {
-            ks = a.k_scale[static_cast<int64_t>(id) * a.heads + cur.h];
-            vs = a.v_scale[static_cast<int64_t>(id) * a.heads + cur.h];
+          if (!is_v) {
+            const bool here = id >= 0;
+            const int64_t at = static_cast<int64_t>(here ? id : 0) * a.heads + cur.h;
+            const float k = here ? a.k_scale[at] : 0.0f, v = here ? a.v_scale[at] : 0.0f;
+            const float lv = here ? log2f(v) : -INFINITY;
+            const int live = here ? min(16, cur.lim - (kt + j + (lane >> 3)) * kQtKeys - (lane & 7) * 16) : 0;
+            float low = lv, high = lv;
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) {
+              low = fminf(low, __shfl_xor_sync(~0u, low, d));
+              high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
+            }
+            const uint32_t full = __ballot_sync(~0u, live == 16) >> (lane & 24) & 0xffu;
+            if (j + (lane >> 3) < tiles) {
+              QtMeta& m = metas[(n0 + j + (lane >> 3)) % kQtMeta];
+              const int g = lane & 7;
+              m.c[g] = k * a.scale_log2;
+              m.lv[g] = lv;
+              m.iv[g] = 1.0f / v;
+              m.live[g] = live;
+              if (g == 0) {
+                m.full = full == 0xffu;
+                m.lv_low = low;
+                m.lv_high = high;
+              }
+            }
+            __syncwarp();
+            if ((lane & 7) == 0 && j + (lane >> 3) < tiles) mbar_arrive(&bar.meta_full[(n0 + j + (lane >> 3)) % kQtMeta]);
           }
         }
         const uint32_t nj = n0 + j;
-        const int from = (j & 3) * 8 + (lane & 7);
-        const int pg = __shfl_sync(~0u, id, from);
+        const int pg = __shfl_sync(~0u, id, (j & 3) * 8 + (lane & 7));
         const int tok = (kt + j) * kQtKeys + (lane & 7) * 16;
-        if (!__all_sync(~0u, wait(&bar.raw_empty[is_v], (nj & 1) ^ 1))) return false;
-        if (!is_v) {
-          QtMeta& m = metas[nj % kQtMeta];
-          const float k = __shfl_sync(~0u, ks, from), v = __shfl_sync(~0u, vs, from);
-          const float lv = pg >= 0 ? log2f(v) : -INFINITY;
-          const int live = pg >= 0 ? min(16, cur.lim - tok) : 0;
-          float low = lv, high = lv;
-#pragma unroll
-          for (int d = 1; d < 8; d <<= 1) {
-            low = fminf(low, __shfl_xor_sync(~0u, low, d));
-            high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
-          }
-          const uint32_t full = __ballot_sync(~0u, live == 16) & 0xffu;
-          if (lane < 8) {
-            m.c[lane] = k * a.scale_log2;
-            m.lv[lane] = lv;
-            m.iv[lane] = 1.0f / v;
-            m.live[lane] = live;
-          }
-          if (lane == 0) {
-            m.full = full == 0xffu;
-            m.lv_low = low;
-            m.lv_high = high;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.meta_full[nj % kQtMeta]);
-        }
         const uint32_t have = __ballot_sync(~0u, pg >= 0) & 0xffu;
+        const uint8_t* src = (is_v ? a.v_cache : a.k_cache) +
+                             (((static_cast<int64_t>(pg) * a.heads + cur.h) << block_shift) + (tok & (a.block - 1))) * kDim;
+        if (!__all_sync(~0u, wait(&bar.raw_empty[is_v], (nj & 1) ^ 1))) return false;
         if (lane == 0) mbar_expect_tx(&bar.raw_full[is_v], __popc(have) * 16 * kDim);
         __syncwarp();
         if (lane < 8 && pg >= 0)
-          bulk_load(smem_at + Cfg::kCodes + is_v * Cfg::kRaw + lane * 16 * kDim,
-                    (is_v ? a.v_cache : a.k_cache) +
-                        (((static_cast<int64_t>(pg) * a.heads + cur.h) << block_shift) + (tok & (a.block - 1))) * kDim,
-                    16 * kDim, &bar.raw_full[is_v]);
+          bulk_load(smem_at + Cfg::kCodes + is_v * Cfg::kRaw + lane * 16 * kDim, src, 16 * kDim, &bar.raw_full[is_v]);
         return true;
       };
-      if (warp == 8) ok = load(0, false) && load(0, true);
+      if (ew < 2) ok = load(0, ew);
       for (int j = 0; j < tiles && ok; ++j, ++n) {
         const int st = n % Cfg::kStages;
         const uint32_t round = n / Cfg::kStages;
@@ -389,7 +384,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
           mbar_arrive(&bar.k_full[st]);
           mbar_arrive(&bar.raw_empty[0]);
         }
-        if (warp == 8 && j + 1 < tiles) ok = load(j + 1, false);
+        if (ew == 0 && j + 1 < tiles) ok = load(j + 1, 0);
         // V: a dimension's 16 tokens to two chunks of its row of V^T; tokens nobody sees become 0, since 0 times
         // whatever they hold need not be 0
         ok = ok && wait(&bar.raw_full[1], n & 1) && wait(&bar.v_empty[st], (round & 1) ^ 1);
@@ -405,15 +400,12 @@ __global__ void __launch_bounds__(kQtThreads, 1) cache_attn_tiles_kernel(const C
           mbar_arrive(&bar.v_full[st]);
           mbar_arrive(&bar.raw_empty[1]);
         }
-        if (warp == 8 && j + 1 < tiles) ok = load(j + 1, true);
+        if (ew == 1 && j + 1 < tiles) ok = load(j + 1, 1);
         ok = __all_sync(~0u, ok && !*failed);
       }
       advance(tiles);
     }
-    if (!ok && warp == 8) {  // copies under way land before the shared memory is given up (bounded waits)
-      mbar_wait(&bar.raw_full[0], n & 1);
-      mbar_wait(&bar.raw_full[1], n & 1);
-    }
+    if (!ok && ew < 2) mbar_wait(&bar.raw_full[ew], n & 1);  // a copy under way lands first (a bounded wait)
   } else {
     // ------------------------------------------------------------ softmax
     const int X = warp >> 2;
