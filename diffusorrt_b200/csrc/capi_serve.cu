@@ -152,7 +152,7 @@ extern "C" int drt_cache_append(const void* k, int64_t k_row, int64_t k_head, co
   a.rows = rows;
   a.heads = heads;
   a.block = block;
-  a.group = rows <= kAppendSingleRows ? 1 : 16;
+  a.group = rows <= kAppendFewRows ? kAppendThreads / 32 : kAppendGroup;
   a.blocks = blocks;
   a.k_cache = static_cast<uint8_t*>(k_cache);
   a.v_cache = static_cast<uint8_t*>(v_cache);

@@ -10,7 +10,6 @@
 // A code is int8 in [-127, 127] or a finite float8 e4m3 (|code| <= 448). Slot = block id * block + offset.
 #pragma once
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "common.cuh"
 
@@ -19,19 +18,34 @@ namespace drt {
 enum CacheCode : int { CACHE_INT8 = 0, CACHE_E4M3 = 1 };
 
 // ---------------------------------------------------------------- 8-bit codes
-template <int kCode>
-__device__ __forceinline__ float code_to_f32(uint32_t byte) {
-  if constexpr (kCode == CACHE_INT8) return static_cast<float>(static_cast<int8_t>(byte));
-  __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
-  return __half2float(__half(h));
+// Two f32 as e4m3 (nearest even, saturating), x in the low byte; and two e4m3 as f32.
+__device__ __forceinline__ uint32_t f32_to_e4m3x2(float x, float y) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y), "f"(x));
+  return r;
 }
-// Round to nearest even onto the codes, saturating; NaN becomes 0.
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t w) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(w)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&r));
+}
+// Two values rounded to nearest even onto the codes, saturating, NaN to 0: x in the low byte.
 template <int kCode>
-__device__ __forceinline__ uint32_t f32_to_code(float v) {
-  if (v != v) v = 0.0f;
+__device__ __forceinline__ uint32_t f32_to_codes(float x, float y) {
+  x = x == x ? x : 0.0f;
+  y = y == y ? y : 0.0f;
+  if constexpr (kCode == CACHE_INT8) {
+    const int i = __float2int_rn(fminf(127.0f, fmaxf(-127.0f, x))), j = __float2int_rn(fminf(127.0f, fmaxf(-127.0f, y)));
+    return (static_cast<uint32_t>(i) & 0xffu) | ((static_cast<uint32_t>(j) & 0xffu) << 8);
+  }
+  return f32_to_e4m3x2(x, y);
+}
+// Two codes (the low bytes of w) as values.
+template <int kCode>
+__device__ __forceinline__ float2 codes_to_f32(uint32_t w) {
   if constexpr (kCode == CACHE_INT8)
-    return static_cast<uint32_t>(__float2int_rn(fminf(127.0f, fmaxf(-127.0f, v)))) & 0xffu;
-  return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+    return make_float2(static_cast<float>(static_cast<int8_t>(w)), static_cast<float>(static_cast<int8_t>(w >> 8)));
+  return e4m3x2_to_f32(w);
 }
 template <int kCode>
 __device__ __forceinline__ constexpr float code_max() {
@@ -254,7 +268,7 @@ __global__ void __launch_bounds__(256) plan_slots_kernel(const PlanArgs a) {
 }
 
 // ---------------------------------------------------------------- append
-// Rows with consecutive slots inside one block are a run; one CTA takes a run of one head of K or of V:
+// Rows with consecutive slots inside one block are a run; one warp or CTA takes a run of one head of K or of V:
 //   amax = max |x| over the run (finite values), s = max(amax / Q, s_old if the run does not begin the block)
 //   code = rn(x / s); the block's other tokens become rn(code * (s_old / s)) when s has grown
 // A run that begins a block starts it anew: what the block held before is gone.
@@ -262,7 +276,8 @@ __global__ void __launch_bounds__(256) plan_slots_kernel(const PlanArgs a) {
 // differs from the quotient's only within 2^-22 of a tie); a scale below 2^-100 divides instead, since its
 // reciprocal leaves the range.
 constexpr int kAppendThreads = 256;
-constexpr int kAppendSingleRows = 1024;  // up to here a CTA per row: single tokens of many requests are runs of one
+constexpr int kAppendGroup = 32;  // rows whose runs a CTA looks for when the call has many, a lane each
+constexpr int kAppendFewRows = 1024;  // up to here eight rows to a CTA, a warp each if they are runs of their own
 
 struct AppendArgs {
   const void *k, *v;
@@ -276,129 +291,291 @@ struct AppendArgs {
   int vec;         // every row of k and v starts on a 16-byte boundary
 };
 
+// Four finite products |v| <= Q (1 + 2^-22) as codes. int8: adding 1.5 2^23 rounds to an integer (ties to even) in the
+// low byte, and none leaves [-127, 127]. (The callers' products are __fmul_rn: fused with this addition they would be
+// rounded once instead of twice.)
 template <int kCode>
-__device__ __forceinline__ uint32_t append_code(float x, float s, float inv) {
-  if (s == 0.0f) return 0;
-  return f32_to_code<kCode>(s < 0x1p-100f ? __fdiv_rn(x, s) : x * inv);
+__device__ __forceinline__ uint32_t finite_codes4(float v0, float v1, float v2, float v3) {
+  if constexpr (kCode == CACHE_INT8) {
+    constexpr float kRound = 12582912.0f;
+    const uint32_t lo = __byte_perm(__float_as_uint(v0 + kRound), __float_as_uint(v1 + kRound), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(v2 + kRound), __float_as_uint(v3 + kRound), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
+  return f32_to_e4m3x2(v0, v1) | f32_to_e4m3x2(v2, v3) << 16;
+}
+__device__ __forceinline__ float2 pair_f32(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ float2 pair_f32(uint32_t u, __nv_bfloat16) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+// max(m, |x|) of two packed values; a NaN stays.
+__device__ __forceinline__ uint32_t pair_max(uint32_t m, uint32_t x, __half) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&m), __habs2(*reinterpret_cast<const __half2*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pair_max(uint32_t m, uint32_t x, __nv_bfloat16) {
+  const __nv_bfloat162 r =
+      __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&m), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x)));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// A run of one or two rows by one warp, as single tokens of many requests are: eight values a lane. V's codes are
+// stored byte by byte, since nothing else of their groups changes unless the scale grows.
+template <typename T, int kDim, int kCode>
+__device__ __forceinline__ void append_few(const AppendArgs& a, const T* x, int64_t ld, bool is_v, int h, int lane, int t, int slot,
+                                           int m, int shift) {
+  constexpr int kLanes = kDim / 8;  // of a row
+  const int off = slot & (a.block - 1), r = lane / kLanes, c = (lane % kLanes) * 8;
+  const int64_t at = static_cast<int64_t>(slot >> shift) * a.heads + h;
+  float* scale = (is_v ? a.v_scale : a.k_scale) + at;
+  const float s_old = off > 0 ? *scale : 0.0f;
+  float v[8];
+  float amax = 0.0f;
+  const bool mine = r < m;
+  if (mine) {
+    __align__(16) T e[8];
+    const T* src = x + (t + r) * ld + c;
+    if (a.vec) {
+      *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(src));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = src[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = cache_in_f32(e[j]);
+      if (fabsf(v[j]) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(v[j]));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+  const float s = fmaxf(__fdiv_rn(amax, code_max<kCode>()), s_old);
+  const bool divide = s > 0.0f && s < 0x1p-100f;
+  const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+  auto quant = [&](float y) { return divide ? __fdiv_rn(y, s) : s > 0.0f ? __fmul_rn(y, inv) : 0.0f; };
+  uint8_t* dst = (is_v ? a.v_cache : a.k_cache) + at * (static_cast<int64_t>(a.block) * kDim);
+  if (off > 0 && s > s_old) {  // every code of the block under the new scale; the run's own follow
+    const float ratio = __fdiv_rn(s_old, s);
+    auto again4 = [&](uint32_t w) {
+      const float2 p = codes_to_f32<kCode>(w & 0xffffu), q = codes_to_f32<kCode>(w >> 16);
+      return f32_to_codes<kCode>(p.x * ratio, p.y * ratio) | f32_to_codes<kCode>(q.x * ratio, q.y * ratio) << 16;
+    };
+    uint4* p = reinterpret_cast<uint4*>(dst);
+#pragma unroll 4
+    for (int i = lane; i < a.block * kDim / 16; i += 32) {
+      const uint4 o = p[i];
+      p[i] = make_uint4(again4(o.x), again4(o.y), again4(o.z), again4(o.w));
+    }
+    __syncwarp();
+  }
+  if (mine) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = f32_to_codes<kCode>(quant(v[2 * j]), quant(v[2 * j + 1]));
+    const int tok = off + r;
+    if (!is_v) {
+      *reinterpret_cast<uint2*>(dst + tok * kDim + c) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    } else {
+      uint8_t* p = dst + ((tok / 16) * kDim + c) * 16 + tok % 16;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j * 16] = static_cast<uint8_t>(w[j / 2] >> (8 * (j & 1)));
+    }
+  }
+  if (lane == 0) *scale = s;
+}
+
+// A longer run by the CTA. Its rows are read once, eight values a thread and turn: K's stay in registers until the scale is known, V's go to
+// shared memory and are read back by columns, two dimensions of 16 tokens a thread. Runs with an infinity or a NaN, or
+// with a scale below 2^-100, take the checked conversions; the other ones (about five instructions a value) need none.
 template <typename T, int kDim, int kCode>
 __global__ void __launch_bounds__(kAppendThreads) append_cache_kernel(const AppendArgs a) {
-  __shared__ __align__(16) T sx[128 * kDim];
+  constexpr int kPitch = kDim + 8;
+  constexpr int kTurns = 128 * kDim / 8 / kAppendThreads;
+  __shared__ __align__(16) T sx[128 * kPitch];
   __shared__ float red[kAppendThreads / 32];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
   const T* x = static_cast<const T*>(is_v ? a.v : a.k) + h * (is_v ? a.v_head : a.k_head);
   const int64_t ld = is_v ? a.v_row : a.k_row;
   const int64_t total = a.blocks * a.block;
-  const int g0 = blockIdx.x * a.group;
-  for (int t = g0; t < min(g0 + a.group, a.rows); ++t) {
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= total) continue;
-    const int64_t b = slot / a.block;
-    const int off = slot - static_cast<int>(b) * a.block;
-    if (t > 0 && off > 0 && a.slots[t - 1] == slot - 1) continue;  // inside another row's run
-    int m = 1;
-    while (off + m < a.block && t + m < a.rows && a.slots[t + m] == slot + m) ++m;
-    // the run's values into shared memory, and their largest magnitude
-    float amax = 0.0f;
-    auto take = [&](T v) {
-      const float f = fabsf(cache_in_f32(v));
-      if (f <= 3.402823466e38f) amax = fmaxf(amax, f);
-    };
-    if (a.vec) {
-      for (int i = tid; i < m * (kDim / 8); i += kAppendThreads) {
-        const int r = i / (kDim / 8), c = (i % (kDim / 8)) * 8;
-        const uint4 u = *reinterpret_cast<const uint4*>(x + (t + r) * ld + c);
-        *reinterpret_cast<uint4*>(sx + r * kDim + c) = u;
-        const T* e = reinterpret_cast<const T*>(&u);
+  const int g0 = blockIdx.x * a.group, rows = min(a.group, a.rows - g0);
+  // which of the rows begin a run, and of one or two rows or of more: one lane each, in every warp
+  const int shift = 31 - __clz(a.block);
+  bool begins = false;
+  int my_slot = -1, my_rows = 1;
+  if (lane < rows) {
+    const int t = g0 + lane;
+    my_slot = a.slots[t];
+    const int before = t > 0 ? a.slots[t - 1] : -1;
+    const int next = t + 1 < a.rows ? a.slots[t + 1] : -1, third = t + 2 < a.rows ? a.slots[t + 2] : -1;
+    const int off = my_slot & (a.block - 1);
+    begins = my_slot >= 0 && my_slot < total && (off == 0 || before != my_slot - 1);
+    if (off + 1 < a.block && next == my_slot + 1) my_rows = off + 2 < a.block && third == my_slot + 2 ? 3 : 2;
+  }
+  uint32_t few = __ballot_sync(~0u, begins && my_rows <= 2);
+  for (int k = 0; few; ++k, few &= few - 1) {  // dealt to the warps
+    if (k % (kAppendThreads / 32) != warp) continue;
+    const int q = __ffs(few) - 1;
+    append_few<T, kDim, kCode>(a, x, ld, is_v, h, lane, g0 + q, __shfl_sync(~0u, my_slot, q), __shfl_sync(~0u, my_rows, q), shift);
+  }
+  for (uint32_t runs = __ballot_sync(~0u, begins && my_rows > 2); runs; runs &= runs - 1) {
+    const int q = __ffs(runs) - 1, t = g0 + q;
+    const int slot = __shfl_sync(~0u, my_slot, q), off = slot & (a.block - 1);
+    const int64_t b = slot >> shift;
+    int m = 0;  // the run's rows: how far the slots go on by one
+    const int most = min(a.block - off, a.rows - t);
+    for (int i0 = 0; i0 < most; i0 += 32) {
+      const int i = i0 + lane;
+      const uint32_t no = __ballot_sync(~0u, i >= most || a.slots[min(t + i, a.rows - 1)] != slot + i);
+      m = i0 + (no ? __ffs(no) - 1 : 32);
+      if (no) break;
+    }
+    float* scale = (is_v ? a.v_scale : a.k_scale) + b * a.heads + h;
+    const float s_old = off > 0 ? *scale : 0.0f;
+    // ---- the run's values, and their largest magnitude
+    uint4 mine[kTurns];
+    uint32_t packed = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) take(e[j]);
-      }
-    } else {
-      for (int i = tid; i < m * kDim; i += kAppendThreads) {
-        const T v = x[(t + i / kDim) * ld + i % kDim];
-        sx[i] = v;
-        take(v);
+    for (int u = 0; u < kTurns; ++u) {
+      const int i = tid + u * kAppendThreads, r = i / (kDim / 8), c = (i % (kDim / 8)) * 8;
+      mine[u] = make_uint4(0, 0, 0, 0);
+      if (r < m) {
+        if (a.vec) {
+          mine[u] = __ldg(reinterpret_cast<const uint4*>(x + (t + r) * ld + c));
+        } else {
+          __align__(16) T e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = x[(t + r) * ld + c + j];
+          mine[u] = *reinterpret_cast<const uint4*>(e);
+        }
       }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-    if ((tid & 31) == 0) red[tid >> 5] = amax;
-    __syncthreads();
+    for (int u = 0; u < kTurns; ++u) {
+      const int i = tid + u * kAppendThreads, r = i / (kDim / 8), c = (i % (kDim / 8)) * 8;
+      packed = pair_max(packed, mine[u].x, T());
+      packed = pair_max(packed, mine[u].y, T());
+      packed = pair_max(packed, mine[u].z, T());
+      packed = pair_max(packed, mine[u].w, T());
+      if (is_v && r < m) *reinterpret_cast<uint4*>(sx + r * kPitch + c) = mine[u];
+    }
+    auto reduce = [&](float v) {  // the CTA's maximum
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, red[w]);
-    float* scale = (is_v ? a.v_scale : a.k_scale) + b * a.heads + h;
-    const float s_old = off > 0 ? *scale : 0.0f;
+      for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+      if (lane == 0) red[warp] = v;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kAppendThreads / 32; ++w) v = fmaxf(v, red[w]);
+      return v;
+    };
+    const float2 two = pair_f32(packed, T());
+    // a NaN anywhere shows as an infinity here, as an infinity does
+    float amax = reduce(two.x == two.x && two.y == two.y ? fmaxf(two.x, two.y) : INFINITY);
+    const bool finite = amax <= 3.402823466e38f;
+    if (!finite) {
+      float v = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        const uint32_t w[4] = {mine[u].x, mine[u].y, mine[u].z, mine[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = pair_f32(w[j], T());
+          if (fabsf(p.x) <= 3.402823466e38f) v = fmaxf(v, fabsf(p.x));
+          if (fabsf(p.y) <= 3.402823466e38f) v = fmaxf(v, fabsf(p.y));
+        }
+      }
+      __syncthreads();  // red has been read
+      amax = reduce(v);
+    }
     const float s = fmaxf(__fdiv_rn(amax, code_max<kCode>()), s_old);
     const bool grew = off > 0 && s > s_old;
     const float ratio = grew ? __fdiv_rn(s_old, s) : 1.0f;
-    const float inv = __fdiv_rn(1.0f, s);
+    const bool divide = s > 0.0f && s < 0x1p-100f;
+    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    const bool plain = finite && !divide;
+    auto checked4 = [&](float v0, float v1, float v2, float v3) {  // of products already taken
+      return f32_to_codes<kCode>(v0, v1) | f32_to_codes<kCode>(v2, v3) << 16;
+    };
+    auto quant = [&](float v) { return divide ? __fdiv_rn(v, s) : s > 0.0f ? __fmul_rn(v, inv) : 0.0f; };
+    auto again4 = [&](uint32_t w) {  // four codes of the block's other tokens under the new scale
+      const float2 p = codes_to_f32<kCode>(w & 0xffffu), q2 = codes_to_f32<kCode>(w >> 16);
+      return checked4(p.x * ratio, p.y * ratio, q2.x * ratio, q2.y * ratio);
+    };
     uint8_t* dst = (is_v ? a.v_cache : a.k_cache) + (b * a.heads + h) * (static_cast<int64_t>(a.block) * kDim);
     if (!is_v) {
-      // 16 codes of a token at a time; only the run's tokens unless the scale grew
-      const int first = grew ? 0 : off, last = grew ? a.block : off + m;
-      for (int i = tid; i < (last - first) * (kDim / 16); i += kAppendThreads) {
-        const int tok = first + i / (kDim / 16), c = (i % (kDim / 16)) * 16;
-        uint4* p = reinterpret_cast<uint4*>(dst + tok * kDim + c);
-        uint32_t w[4];
-        if (tok >= off && tok < off + m) {
-          const T* e = sx + (tok - off) * kDim + c;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) {
+        const int i = tid + u * kAppendThreads, r = i / (kDim / 8), c = (i % (kDim / 8)) * 8;
+        if (r >= m) continue;
+        const float2 p0 = pair_f32(mine[u].x, T()), p1 = pair_f32(mine[u].y, T());
+        const float2 p2 = pair_f32(mine[u].z, T()), p3 = pair_f32(mine[u].w, T());
+        uint2 w;
+        if (plain) {
+          w.x = finite_codes4<kCode>(__fmul_rn(p0.x, inv), __fmul_rn(p0.y, inv), __fmul_rn(p1.x, inv), __fmul_rn(p1.y, inv));
+          w.y = finite_codes4<kCode>(__fmul_rn(p2.x, inv), __fmul_rn(p2.y, inv), __fmul_rn(p3.x, inv), __fmul_rn(p3.y, inv));
+        } else {
+          w.x = checked4(quant(p0.x), quant(p0.y), quant(p1.x), quant(p1.y));
+          w.y = checked4(quant(p2.x), quant(p2.y), quant(p3.x), quant(p3.y));
+        }
+        *reinterpret_cast<uint2*>(dst + (off + r) * kDim + c) = w;
+      }
+      if (grew)  // the block's other tokens
+        for (int i = tid; i < (a.block - m) * (kDim / 16); i += kAppendThreads) {
+          const int j = i / (kDim / 16), tok = j < off ? j : j + m;
+          uint4* p = reinterpret_cast<uint4*>(dst + tok * kDim + (i % (kDim / 16)) * 16);
+          const uint4 o = *p;
+          *p = make_uint4(again4(o.x), again4(o.y), again4(o.z), again4(o.w));
+        }
+    } else {
+      // 16 tokens of two dimensions at a time; groups that the run fills in part keep their other codes
+      const int first = grew ? 0 : off / 16, last = grew ? a.block / 16 : (off + m + 15) / 16;
+      for (int i = tid; i < (last - first) * (kDim / 2); i += kAppendThreads) {
+        const int grp = first + i / (kDim / 2), d = (i % (kDim / 2)) * 2;
+        uint4* p = reinterpret_cast<uint4*>(dst + (grp * kDim + d) * 16);
+        const int lo = off - grp * 16, hi = lo + m;  // the run's tokens within this group
+        uint32_t w[2][4];
+        if (plain && lo <= 0 && hi >= 16) {
+          const T* e = sx - lo * kPitch + d;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            w[j] = 0;
+            float2 v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) w[j] |= append_code<kCode>(cache_in_f32(e[j * 4 + q]), s, inv) << (8 * q);
+            for (int k = 0; k < 4; ++k) v[k] = pair_f32(*reinterpret_cast<const uint32_t*>(e + (j * 4 + k) * kPitch), T());
+            w[0][j] = finite_codes4<kCode>(__fmul_rn(v[0].x, inv), __fmul_rn(v[1].x, inv), __fmul_rn(v[2].x, inv), __fmul_rn(v[3].x, inv));
+            w[1][j] = finite_codes4<kCode>(__fmul_rn(v[0].y, inv), __fmul_rn(v[1].y, inv), __fmul_rn(v[2].y, inv), __fmul_rn(v[3].y, inv));
           }
         } else {
-          const uint4 o = *p;
-          const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+          const uint4 o0 = p[0], o1 = p[1];
+          const uint32_t old[2][4] = {{o0.x, o0.y, o0.z, o0.w}, {o1.x, o1.y, o1.z, o1.w}};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = 0;
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              w[j] |= f32_to_code<kCode>(code_to_f32<kCode>((ow[j] >> (8 * q)) & 0xff) * ratio) << (8 * q);
-          }
+            for (int j = 0; j < 4; ++j) {
+              w[k][j] = grew ? again4(old[k][j]) : old[k][j];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int tok = j * 4 + e;
+                if (tok >= lo && tok < hi) {
+                  const uint32_t c = f32_to_codes<kCode>(quant(cache_in_f32(sx[(tok - lo) * kPitch + d + k])), 0.0f) & 0xffu;
+                  w[k][j] = (w[k][j] & ~(0xffu << (8 * e))) | c << (8 * e);
+                }
+              }
+            }
         }
-        *p = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    } else {
-      // 16 tokens of a dimension at a time; chunks that the run fills in part keep their other codes
-      const int first = grew ? 0 : off / 16, last = grew ? a.block / 16 : (off + m + 15) / 16;
-      for (int i = tid; i < (last - first) * kDim; i += kAppendThreads) {
-        const int grp = first + i / kDim, d = i % kDim;
-        uint4* p = reinterpret_cast<uint4*>(dst + (grp * kDim + d) * 16);
-        const int lo = off - grp * 16, hi = lo + m;  // the run's tokens within this chunk
-        uint32_t w[4];
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (lo > 0 || hi < 16) o = *p;
-        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = 0;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int tok = j * 4 + q;
-            uint32_t c = (ow[j] >> (8 * q)) & 0xff;
-            if (tok >= lo && tok < hi) c = append_code<kCode>(cache_in_f32(sx[(tok - lo) * kDim + d]), s, inv);
-            else if (grew) c = f32_to_code<kCode>(code_to_f32<kCode>(c) * ratio);
-            w[j] |= c << (8 * q);
-          }
-        }
-        *p = make_uint4(w[0], w[1], w[2], w[3]);
+        p[0] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+        p[1] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
       }
     }
-    __syncthreads();  // every thread has read the old scale, and sx may be filled again
+    __syncthreads();  // every thread has read the old scale and the reduction, and sx may be filled again
     if (tid == 0) *scale = s;
   }
 }
 
 // ---------------------------------------------------------------- read back
 // Values scale * code of the listed slots, rounded once to T; a slot outside the cache gives zeros.
-// One CTA takes 16 list entries of one head. V's codes of one token lie 16 bytes apart, so 16 entries that
-// are one aligned group are read as one 16-byte load for each dimension.
+// One CTA takes 16 list entries of one head. V's codes of one token lie 16 bytes apart, so 16 entries that are one
+// aligned group are read eight tokens of a dimension at a time.
 constexpr int kReadThreads = 128;
 constexpr int kReadRows = 16;
 
@@ -414,70 +591,78 @@ struct ReadArgs {
 template <typename T, int kDim, int kCode>
 __global__ void __launch_bounds__(kReadThreads) read_cache_kernel(const ReadArgs a) {
   __shared__ int slot_s[kReadRows];
+  __shared__ float ks_s[kReadRows], vs_s[kReadRows];
+  __shared__ int64_t plane_s[kReadRows];  // the entry's block and head in the cache, in bytes
   const int tid = threadIdx.x;
   const int r0 = blockIdx.x * kReadRows, h = blockIdx.y;
   const int64_t total = a.blocks * a.block;
   const int n = min(kReadRows, a.rows - r0);
-  if (tid < kReadRows) {
+  bool group = false;
+  if (tid < 32) {
     int s = tid < n ? a.slots[r0 + tid] : -1;
     if (s >= total) s = -1;
-    slot_s[tid] = s;
-  }
-  __syncthreads();
-  const int64_t plane = static_cast<int64_t>(a.block) * kDim;
-  const int s0 = slot_s[0];
-  bool group = n == kReadRows && s0 >= 0 && s0 % 16 == 0;
-  for (int i = 1; i < n; ++i) group = group && slot_s[i] == s0 + i;
-  constexpr int kPairs = kDim / 2;            // a thread writes two dimensions of a row
-  constexpr int kRowsAtOnce = kReadThreads / kPairs;
-  const int d = (tid % kPairs) * 2, sub = tid / kPairs;
-  T* ko = static_cast<T*>(a.k_out);
-  T* vo = static_cast<T*>(a.v_out);
-  uint4 c0 = make_uint4(0, 0, 0, 0), c1 = c0;
-  if (group) {
-    const int64_t b = s0 / a.block;
-    const uint8_t* p = a.v_cache + (b * a.heads + h) * plane + ((s0 - b * a.block) / 16 * kDim + d) * 16;
-    c0 = *reinterpret_cast<const uint4*>(p);
-    c1 = *reinterpret_cast<const uint4*>(p + 16);
-  }
-  const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-  for (int j = 0; j < kReadRows / kRowsAtOnce; ++j) {
-    const int i = kRowsAtOnce == 1 ? j : j * kRowsAtOnce + sub;
-    if (i >= n) continue;
-    const int s = slot_s[i];
-    float kx = 0.0f, ky = 0.0f, vx = 0.0f, vy = 0.0f;
-    if (s >= 0) {
-      const int64_t b = s / a.block;
-      const int off = s - static_cast<int>(b) * a.block;
-      const float ks = a.k_scale[b * a.heads + h], vs = a.v_scale[b * a.heads + h];
-      const uint32_t kk = *reinterpret_cast<const uint16_t*>(a.k_cache + (b * a.heads + h) * plane + off * kDim + d);
-      kx = code_to_f32<kCode>(kk & 0xff) * ks;
-      ky = code_to_f32<kCode>(kk >> 8) * ks;
-      uint32_t v0, v1;
-      if (group) {
-        uint32_t u0 = w0[0], u1 = w1[0];
-#pragma unroll
-        for (int q = 1; q < 4; ++q)
-          if ((i >> 2) == q) {
-            u0 = w0[q];
-            u1 = w1[q];
-          }
-        v0 = (u0 >> (8 * (i & 3))) & 0xff;
-        v1 = (u1 >> (8 * (i & 3))) & 0xff;
-      } else {
-        const uint8_t* p = a.v_cache + (b * a.heads + h) * plane + (off / 16 * kDim + d) * 16 + off % 16;
-        v0 = p[0];
-        v1 = p[16];
-      }
-      vx = code_to_f32<kCode>(v0) * vs;
-      vy = code_to_f32<kCode>(v1) * vs;
+    const int s0 = __shfl_sync(~0u, s, 0);
+    const int64_t b = s >= 0 ? s / a.block : 0;
+    if (tid < kReadRows) {
+      slot_s[tid] = s >= 0 ? s - static_cast<int>(b) * a.block : -1;  // offset within the block
+      plane_s[tid] = (b * a.heads + h) * (static_cast<int64_t>(a.block) * kDim);
+      ks_s[tid] = s >= 0 ? a.k_scale[b * a.heads + h] : 0.0f;
+      vs_s[tid] = s >= 0 ? a.v_scale[b * a.heads + h] : 0.0f;
     }
-    const int64_t at = (static_cast<int64_t>(r0 + i) * a.heads + h) * kDim + d;
-    ko[at] = cache_out<T>(kx);
-    ko[at + 1] = cache_out<T>(ky);
-    vo[at] = cache_out<T>(vx);
-    vo[at + 1] = cache_out<T>(vy);
+    group = __all_sync(~0u, tid >= kReadRows || (s0 >= 0 && s0 % 16 == 0 && s == s0 + tid));
+  }
+  group = __syncthreads_or(group);
+  // K: 16 dimensions of an entry at a time
+  for (int i = tid; i < n * (kDim / 16); i += kReadThreads) {
+    const int e = i / (kDim / 16), c = (i % (kDim / 16)) * 16, off = slot_s[e];
+    const float s = ks_s[e];
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (off >= 0) u = *reinterpret_cast<const uint4*>(a.k_cache + plane_s[e] + off * kDim + c);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __align__(16) T o[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 p = codes_to_f32<kCode>((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+      o[2 * j] = cache_out<T>(p.x * s);
+      o[2 * j + 1] = cache_out<T>(p.y * s);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (static_cast<int64_t>(r0 + e) * a.heads + h) * kDim + c);
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) dst[j] = reinterpret_cast<const uint4*>(o)[j];
+  }
+  // V: two dimensions of a half group's eight tokens at a time
+  constexpr int kPairs = kDim / 2;
+  for (int i = tid; i < 2 * kPairs; i += kReadThreads) {
+    const int d = (i % kPairs) * 2, half = i / kPairs;
+    uint32_t w0[2] = {0, 0}, w1[2] = {0, 0};
+    if (group) {
+      const uint8_t* p = a.v_cache + plane_s[0] + (slot_s[0] / 16 * kDim + d) * 16 + half * 8;
+      const uint2 u0 = *reinterpret_cast<const uint2*>(p), u1 = *reinterpret_cast<const uint2*>(p + 16);
+      w0[0] = u0.x;
+      w0[1] = u0.y;
+      w1[0] = u1.x;
+      w1[1] = u1.y;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = half * 8 + j;
+      if (e >= n) break;
+      const int off = slot_s[e];
+      uint32_t pair = ((w0[j >> 2] >> (8 * (j & 3))) & 0xffu) | ((w1[j >> 2] >> (8 * (j & 3))) & 0xffu) << 8;
+      if (!group && off >= 0) {
+        const uint8_t* p = a.v_cache + plane_s[e] + (off / 16 * kDim + d) * 16 + off % 16;
+        pair = p[0] | static_cast<uint32_t>(p[16]) << 8;
+      }
+      const float2 v = codes_to_f32<kCode>(pair);
+      const float s = vs_s[e];
+      T* dst = static_cast<T*>(a.v_out) + (static_cast<int64_t>(r0 + e) * a.heads + h) * kDim + d;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(dst) = make_float2(v.x * s, v.y * s);
+      } else {
+        __align__(4) T o[2] = {cache_out<T>(v.x * s), cache_out<T>(v.y * s)};
+        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(o);
+      }
+    }
   }
 }
 
