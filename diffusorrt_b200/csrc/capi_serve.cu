@@ -366,7 +366,7 @@ cudaError_t run_logprobs(const LogprobArgs& a, cudaStream_t st) {
   cudaError_t e = launch(logprob_stats_kernel<T>, dim3(static_cast<unsigned>(a.rows) * a.slices), dim3(kLpThreads), 0, st, false, a);
   if (e != cudaSuccess) return e;
   const size_t smem = a.top > 0 ? kLpCands * 8 + static_cast<size_t>(a.segs) * 4 : 0;
-  return launch(logprob_finish_kernel<T>, dim3(a.rows), dim3(kLpThreads), smem, st, true, a);
+  return launch(logprob_finish_kernel<T>, dim3(a.rows), dim3(a.rows <= kLpFinFewRows ? kLpFinFew : kLpFinMany), smem, st, true, a);
 }
 }  // namespace
 
@@ -385,7 +385,8 @@ extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t 
   REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab, "bad selector geometry");
   REQUIRE(dtype == DRT_TYPE_F32 || dtype == DRT_TYPE_BF16 || dtype == DRT_TYPE_F16, "logits must be f32, bf16 or f16");
   REQUIRE(top >= 0 && top <= kLpMaxTop, "top must be in [0, %d]", kLpMaxTop);
-  REQUIRE(std::isfinite(temperature), "temperature must be finite");
+  REQUIRE(std::isfinite(temperature) && (temperature <= 0.0 || temperature >= 1e-30),
+          "temperature must be finite, and at least 1e-30 if positive");
   REQUIRE(exclude_token >= -1 && exclude_token < vocab, "exclude_token outside the vocabulary");
   if (rows == 0) return DRT_OK;
   REQUIRE(logits && scratch && (top == 0 || (top_token && top_logprob)), "null argument");
@@ -408,7 +409,7 @@ extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t 
   a.vocab = vocab;
   a.top = top;
   a.exclude = exclude_token;
-  a.unit = temperature > 0.0 ? static_cast<float>(1.0 / temperature) : 1.0f;
+  a.unit_log2 = static_cast<float>(1.4426950408889634 / (temperature > 0.0 ? temperature : 1.0));
   a.segs = p.segs;
   a.slices = p.slices;
   a.segs_per_slice = p.per;

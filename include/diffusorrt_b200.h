@@ -432,7 +432,7 @@ typedef struct drt_cache_attend_args {
 } drt_cache_attend_args;
 size_t drt_cache_attend_scratch_bytes(int32_t dim);
 int drt_cache_attend(const drt_cache_attend_args* args, void* stream);
-/* Scores of given tokens under softmax(x / T) (T <= 0: no scaling) of rows of logits (DRT_TYPE_*, row r or
+/* Scores of given tokens under softmax(x / T) (T <= 0: no scaling, else T >= 1e-30) of rows of logits (DRT_TYPE_*, row r or
  * row_index[r], row stride ld): logprob[r] of tokens[r] (-inf for a token outside the vocabulary, whose rank
  * is -1), entropy[r] in nats, rank[r] = tokens before it by (logit, lowest id), and the `top` (at most 32)
  * likeliest tokens with their log probabilities in that order, -1 and -inf behind the last of non-zero

@@ -130,6 +130,7 @@ def score(lib, **change):
 @pytest.mark.parametrize("change,message", [
     (dict(logits=None), "null"), (dict(scratch=None), "null"), (dict(tt=None), "null"), (dict(tokens=None), "tokens"),
     (dict(dtype=5), "logits"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(temperature=float("inf")), "temperature"),
+    (dict(temperature=1e-31), "temperature"),
     (dict(exclude=100), "exclude"), (dict(ld=99), "geometry"), (dict(vocab=0), "geometry"), (dict(rows=-1), "geometry"),
     (dict(logits=P + 2), "misaligned")])
 def test_score_refusals(lib, change, message):
