@@ -72,7 +72,7 @@ __device__ __forceinline__ __nv_bfloat16 cache_out<__nv_bfloat16>(float x) { ret
 // ids given back go behind them, so the two never touch one entry. All or nothing: a call that cannot be
 // served writes empty slot maps and a status and changes no table, ring or held count.
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanSlotRows = 1024;   // rows per CTA of plan_slots_kernel
+constexpr int kPlanSlotRows = 1024;   // rows per CTA of 256 threads of plan_slots_kernel
 constexpr int kPlanStageRequests = 4096;  // row starts that a CTA keeps in shared memory
 constexpr int kPlanInlineRows = 4096;  // up to here the first kernel writes the slots itself: one launch
 
@@ -93,29 +93,43 @@ struct PlanArgs {
   int fill_slots;  // 1: this launch writes the slots too
 };
 
-// Last r in [0, n) with first[r] <= t (first is ascending, first[0] <= t): the empty runs before it are passed.
-__device__ __forceinline__ int plan_find(const int* first, int n, int t) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= t) lo = mid;
-    else hi = mid;
+// For each of t, t + step, ...: the last r in [0, n) with first[r] <= t (first is ascending, first[0] <= t), which passes
+// empty runs. The searches go side by side, since a step of one is a shared-memory latency.
+constexpr int kPlanBatch = 4;
+__device__ __forceinline__ void plan_find_batch(const int* first, int n, int t, int step, int* lo) {
+  int hi[kPlanBatch];
+#pragma unroll
+  for (int k = 0; k < kPlanBatch; ++k) {
+    lo[k] = 0;
+    hi[k] = n;
   }
-  return lo;
+  for (int width = n; width > 1; width = (width + 1) >> 1) {
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int mid = (lo[k] + hi[k]) >> 1;
+      if (hi[k] - lo[k] > 1) {
+        if (first[mid] <= t + k * step) lo[k] = mid;
+        else hi[k] = mid;
+      }
+    }
+  }
 }
 
-__device__ __forceinline__ void plan_slot(const PlanArgs& a, const int* first, int total, int t) {
-  int slot = -1, pos = -1;
-  if (t < total) {
-    const int r = plan_find(first, a.requests, t);
-    pos = a.start[r] + (t - first[r]);
-    const int b = pos / a.block;
-    const int64_t id = a.tables[r * a.ld_tables + b];
-    const int64_t s = id * a.block + (pos - b * a.block);
-    if (id >= 0 && s <= INT32_MAX) slot = static_cast<int>(s);
+// Slots and positions of rows t, t + step, ... below `end`.
+__device__ __forceinline__ void plan_slots(const PlanArgs& a, const int* first, int total, int t, int step, int end) {
+  int r[kPlanBatch], pos[kPlanBatch], id[kPlanBatch];
+  plan_find_batch(first, a.requests, t, step, r);
+#pragma unroll
+  for (int k = 0; k < kPlanBatch; ++k) pos[k] = t + k * step < total ? a.start[r[k]] + (t + k * step - first[r[k]]) : -1;
+#pragma unroll
+  for (int k = 0; k < kPlanBatch; ++k) id[k] = pos[k] >= 0 ? a.tables[r[k] * a.ld_tables + pos[k] / a.block] : -1;
+#pragma unroll
+  for (int k = 0; k < kPlanBatch; ++k) {
+    if (t + k * step >= end) break;
+    const int64_t s = static_cast<int64_t>(id[k]) * a.block + pos[k] % a.block;
+    a.slots[t + k * step] = id[k] >= 0 && s <= INT32_MAX ? static_cast<int>(s) : -1;
+    a.positions[t + k * step] = pos[k];
   }
-  a.slots[t] = slot;
-  a.positions[t] = pos;
 }
 
 // One CTA: checks, scans, tables and ring; also the slots of a call with few rows.
@@ -224,15 +238,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs
     const int all_n = scan_w[0][31], all_need = scan_w[1][31], all_gone = scan_w[2][31];
     __syncthreads();
     const int live = min(kPlanThreads, a.requests - r0);
-    for (int e = tid; e < all_need; e += kPlanThreads) {
-      const int i = plan_find(sh_need, live, e);
-      a.tables[(r0 + i) * a.ld_tables + sh_held[i] + (e - sh_need[i])] =
-          a.ring[(static_cast<long long>(head) + base_need + e) % a.ring_size];
+    // place e behind `from` in the ring; from is below twice its size, e below it
+    auto in_ring = [&](long long from, int e) {
+      long long p = from + e;
+      while (p >= a.ring_size) p -= a.ring_size;
+      return static_cast<int>(p);
+    };
+    for (int e = tid; e < all_need; e += kPlanThreads * kPlanBatch) {
+      int i[kPlanBatch], id[kPlanBatch];
+#pragma unroll
+      for (int k = 0; k < kPlanBatch; ++k)
+        if (e + k * kPlanThreads < all_need)
+          id[k] = a.ring[in_ring(static_cast<long long>(head) + base_need, e + k * kPlanThreads)];
+      plan_find_batch(sh_need, live, e, kPlanThreads, i);
+#pragma unroll
+      for (int k = 0; k < kPlanBatch; ++k)
+        if (e + k * kPlanThreads < all_need)
+          a.tables[(r0 + i[k]) * a.ld_tables + sh_held[i[k]] + (e + k * kPlanThreads - sh_need[i[k]])] = id[k];
     }
-    for (int e = tid; e < all_gone; e += kPlanThreads) {
-      const int i = plan_find(sh_gone, live, e);
-      a.ring[(static_cast<long long>(head) + available + base_gone + e) % a.ring_size] =
-          a.tables[(r0 + i) * a.ld_tables + (e - sh_gone[i])];
+    for (int e = tid; e < all_gone; e += kPlanThreads * kPlanBatch) {
+      int i[kPlanBatch], id[kPlanBatch];
+      plan_find_batch(sh_gone, live, e, kPlanThreads, i);
+#pragma unroll
+      for (int k = 0; k < kPlanBatch; ++k)
+        if (e + k * kPlanThreads < all_gone)
+          id[k] = a.tables[(r0 + i[k]) * a.ld_tables + (e + k * kPlanThreads - sh_gone[i[k]])];
+#pragma unroll
+      for (int k = 0; k < kPlanBatch; ++k)
+        if (e + k * kPlanThreads < all_gone)
+          a.ring[in_ring(static_cast<long long>(head) + available + base_gone, e + k * kPlanThreads)] = id[k];
     }
     base_n += all_n;
     base_need += all_need;
@@ -248,7 +282,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs
   if (a.fill_slots) {
     __syncthreads();
     const int* first = a.requests <= kPlanThreads ? sh_rows : a.row_start;
-    for (int t = tid; t < a.max_rows; t += kPlanThreads) plan_slot(a, first, base_n, t);
+    for (int t = tid; t < a.max_rows; t += kPlanThreads * kPlanBatch)
+      plan_slots(a, first, base_n, t, kPlanThreads, a.max_rows);
   }
 }
 
@@ -264,7 +299,8 @@ __global__ void __launch_bounds__(256) plan_slots_kernel(const PlanArgs a) {
     __syncthreads();
     first = sh;
   }
-  for (int t = t0 + threadIdx.x; t < min(t0 + kPlanSlotRows, a.max_rows); t += 256) plan_slot(a, first, total, t);
+  const int t = t0 + threadIdx.x, end = min(t0 + kPlanSlotRows, a.max_rows);
+  if (t < end) plan_slots(a, first, total, t, 256, end);
 }
 
 // ---------------------------------------------------------------- append

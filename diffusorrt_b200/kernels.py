@@ -7,6 +7,7 @@ the token scorer (select_logprobs).
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import NamedTuple
@@ -228,11 +229,12 @@ def _check_ints(t, name: str, index: int, n: int | None = None) -> None:
 
 def _check_tables(t, index: int, n: int) -> tuple[int, int]:
     """(width, row stride) of the block tables."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is _I32 and t.get_device() == index and t.dim() == 2 and t.size(0) == n
-            and t.stride(1) == 1 and (n <= 1 or t.stride(0) >= t.size(1))):
-        raise ValueError(f"tables must be an int32 [{n}, width] tensor with contiguous rows on cuda:{index}")
-    width = t.size(1)
-    return width, max(t.stride(0), width)
+    if isinstance(t, torch.Tensor) and t.dtype is _I32 and t.get_device() == index and t.dim() == 2:
+        rows, width = t.shape
+        ld, step = t.stride()
+        if rows == n and step == 1 and (n <= 1 or ld >= width):
+            return width, max(ld, width)
+    raise ValueError(f"tables must be an int32 [{n}, width] tensor with contiguous rows on cuda:{index}")
 
 
 def _launch(index: int, stream: torch.cuda.Stream | None, made, fn, *args) -> None:
@@ -306,7 +308,7 @@ def plan_cache(start: torch.Tensor, count: torch.Tensor, held: torch.Tensor, tab
     else:
         _check_ints(ring_state_out, "ring_state_out", index, 2)
     made = torch.empty(2 * n + 2 * max_rows + 2, dtype=_I32, device=start.device)
-    row_start, slots, positions, lengths, status = made.split((n + 1, max_rows, max_rows, n, 1))
+    row_start, slots, positions, lengths, status = made.split_with_sizes((n + 1, max_rows, max_rows, n, 1))
     p = made.data_ptr()
     _launch(index, stream, (made,), _lib.load().drt_cache_plan, start.data_ptr(), count.data_ptr(), held.data_ptr(),
             held_out.data_ptr(), n, tables.data_ptr(), ld, width, block_size, ring.data_ptr(), ring.numel(),
@@ -329,8 +331,9 @@ def cache_q8(blocks: int, kv_heads: int, block_size: int, dim: int = 128, *, dty
 
 def _cache_args(k_cache, v_cache, k_scale, v_scale, index: int):
     """(blocks, kv_heads, block, dim, code) of a cache on device `index`."""
-    if not all(isinstance(t, torch.Tensor) and t.get_device() == index and t.is_contiguous()
-               for t in (k_cache, v_cache, k_scale, v_scale)):
+    for t in (k_cache, v_cache, k_scale, v_scale):
+        if isinstance(t, torch.Tensor) and t.get_device() == index and t.is_contiguous():
+            continue
         raise ValueError(f"the cache must be contiguous tensors on {'the CPU' if index < 0 else f'cuda:{index}'}")
     code = _CODES.get(k_cache.dtype)
     if code is None or v_cache.dtype is not k_cache.dtype:
@@ -480,6 +483,12 @@ class TokenScores(NamedTuple):
     top_logprob: torch.Tensor  # f32 [rows, top]
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprob_bytes(n: int, vocab: int, typ: int, index: int) -> int:
+    with torch.cuda.device(index):
+        return int(_lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ))
+
+
 def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, temperature: float = 0.0,
                     exclude_token: int = -1, row_index: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
                     stream: torch.cuda.Stream | None = None) -> TokenScores:
@@ -502,11 +511,7 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
         raise ValueError("one token per logits row")
     if not 0 <= top <= 32:
         raise ValueError("top must be in [0, 32]")
-    if torch.cuda.current_device() == index:
-        size = _lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ)
-    else:
-        with torch.cuda.device(index):
-            size = _lib.load().drt_selector_logprobs_scratch_bytes(n, vocab, typ)
+    size = _logprob_bytes(n, vocab, typ, index)
     words = n * (3 + 2 * top)
     # outputs in one allocation, the call's scratch in front of them
     own = (size + 3) // 4 if scratch is None else 0
@@ -514,8 +519,8 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     if scratch is not None and not (scratch.get_device() == index and scratch.is_contiguous()
                                     and scratch.numel() * scratch.element_size() >= size):
         raise ValueError(f"scratch must hold {size} bytes")
-    _, logprob, entropy, top_logprob, whole = made.split((own, n, n, n * top, n * (1 + top)))
-    rank, top_token = whole.view(_I32).split((n, n * top))
+    _, logprob, entropy, top_logprob, whole = made.split_with_sizes((own, n, n, n * top, n * (1 + top)))
+    rank, top_token = whole.view(_I32).split_with_sizes((n, n * top))
     p = made.data_ptr()
     at = p + 4 * own
     _launch(index, stream, (made,) if scratch is None else (made, scratch), _lib.load().drt_selector_logprobs,
