@@ -93,50 +93,82 @@ struct PlanArgs {
   int fill_slots;  // 1: this launch writes the slots too
 };
 
-// For each of t, t + step, ...: the last r in [0, n) with first[r] <= t (first is ascending, first[0] <= t), which passes
-// empty runs. The searches go side by side, since a step of one is a shared-memory latency.
-constexpr int kPlanBatch = 4;
-__device__ __forceinline__ void plan_find_batch(const int* first, int n, int t, int step, int* lo) {
-  int hi[kPlanBatch];
-#pragma unroll
-  for (int k = 0; k < kPlanBatch; ++k) {
-    lo[k] = 0;
-    hi[k] = n;
-  }
-  for (int width = n; width > 1; width = (width + 1) >> 1) {
-#pragma unroll
-    for (int k = 0; k < kPlanBatch; ++k) {
-      const int mid = (lo[k] + hi[k]) >> 1;
-      if (hi[k] - lo[k] > 1) {
-        if (first[mid] <= t + k * step) lo[k] = mid;
-        else hi[k] = mid;
-      }
-    }
-  }
+// Position p of a request whose table is `table`: its slot, -1 for an entry that is not a block.
+__device__ __forceinline__ int plan_slot(const PlanArgs& a, const int* table, int p) {
+  const int b = p / a.block, id = table[b];
+  const int64_t s = static_cast<int64_t>(id) * a.block + (p - b * a.block);
+  return id >= 0 && s <= INT32_MAX ? static_cast<int>(s) : -1;
 }
 
-// Slots and positions of rows t, t + step, ... below `end`.
-__device__ __forceinline__ void plan_slots(const PlanArgs& a, const int* first, int total, int t, int step, int end) {
-  int r[kPlanBatch], pos[kPlanBatch], id[kPlanBatch];
-  plan_find_batch(first, a.requests, t, step, r);
-#pragma unroll
-  for (int k = 0; k < kPlanBatch; ++k) pos[k] = t + k * step < total ? a.start[r[k]] + (t + k * step - first[r[k]]) : -1;
-#pragma unroll
-  for (int k = 0; k < kPlanBatch; ++k) id[k] = pos[k] >= 0 ? a.tables[r[k] * a.ld_tables + pos[k] / a.block] : -1;
-#pragma unroll
-  for (int k = 0; k < kPlanBatch; ++k) {
-    if (t + k * step >= end) break;
-    const int64_t s = static_cast<int64_t>(id[k]) * a.block + pos[k] % a.block;
-    a.slots[t + k * step] = id[k] >= 0 && s <= INT32_MAX ? static_cast<int>(s) : -1;
-    a.positions[t + k * step] = pos[k];
+// Last r in [lo, n) with first[r] <= t (first is ascending, first[lo] <= t): runs without rows are passed.
+__device__ __forceinline__ int plan_find(const int* first, int lo, int n, int t) {
+  for (int i = 0; i < 4; ++i) {  // rows lie close: a few steps first
+    if (lo + 1 >= n || first[lo + 1] > t) return lo;
+    ++lo;
   }
+  int hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// store(i, k, load(i, k)) for k < size[i + 1] - size[i] of every i < n (n <= kPlanThreads, size ascending): sizes up to 2
+// by a thread, up to 256 by a warp, larger ones by the CTA. Eight loads are under way before their stores: the compiler
+// may not move a load over a store that might change it, and one at a time would cost a memory latency each.
+template <typename L, typename S>
+__device__ __forceinline__ void plan_for_each(const int* size, int n, uint32_t* big, L&& load, S&& store) {
+  constexpr int kAhead = 8;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int at = tid < n ? size[tid] : 0, mine = tid < n ? size[tid + 1] - at : 0;
+  if (mine > 0 && mine <= 2) {
+    const int v0 = load(tid, 0), v1 = mine > 1 ? load(tid, 1) : 0;
+    store(tid, 0, v0);
+    if (mine > 1) store(tid, 1, v1);
+  }
+  for (uint32_t some = __ballot_sync(~0u, mine > 2 && mine <= 256); some;) {
+    int i[kAhead], count[kAhead], v[kAhead], most = 0;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int l = some ? __ffs(some) - 1 : 0;
+      i[j] = warp * 32 + l;
+      count[j] = some ? __shfl_sync(~0u, mine, l) : 0;
+      most = max(most, count[j]);
+      some &= some - 1;
+    }
+    for (int k = lane; k < most; k += 32) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j] = k < count[j] ? load(i[j], k) : 0;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (k < count[j]) store(i[j], k, v[j]);
+    }
+  }
+  const uint32_t large = __ballot_sync(~0u, mine > 256);
+  if (lane == 0) big[warp] = large;
+  if (!__syncthreads_or(mine > 256)) return;
+  for (int w = 0; w < kPlanThreads / 32; ++w)
+    for (uint32_t some = big[w]; some; some &= some - 1) {
+      const int i = w * 32 + __ffs(some) - 1, count = size[i + 1] - size[i];
+      for (int k = tid; k < count; k += kAhead * kPlanThreads) {
+        int v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) v[j] = k + j * kPlanThreads < count ? load(i, k + j * kPlanThreads) : 0;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+          if (k + j * kPlanThreads < count) store(i, k + j * kPlanThreads, v[j]);
+      }
+    }
 }
 
 // One CTA: checks, scans, tables and ring; also the slots of a call with few rows.
 __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs a) {
-  __shared__ long long tot[3][32];
+  __shared__ long long tot[3][32], all_of[3];
+  __shared__ uint32_t big[kPlanThreads / 32];
   __shared__ int bad_flag, scan_w[3][32];
-  __shared__ int sh_need[kPlanThreads + 1], sh_gone[kPlanThreads + 1], sh_held[kPlanThreads], sh_rows[kPlanThreads];
+  __shared__ int sh_need[kPlanThreads + 1], sh_gone[kPlanThreads + 1], sh_rows[kPlanThreads + 1], sh_held[kPlanThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) bad_flag = 0;
   __syncthreads();
@@ -170,12 +202,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs
   }
   if (bad) atomicMin(&bad_flag, bad);
   __syncthreads();
-  long long rows = 0, need_all = 0, gone_all = 0;
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    rows += tot[0][w];
-    need_all += tot[1][w];
-    gone_all += tot[2][w];
+  if (warp < 3) {
+    long long v = tot[warp][lane];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    if (lane == 0) all_of[warp] = v;
   }
+  __syncthreads();
+  const long long rows = all_of[0], need_all = all_of[1], gone_all = all_of[2];
   int status = bad_flag;
   if (status == 0 && rows > a.max_rows) status = -3;
   if (status == 0 && available - need_all + gone_all > a.ring_size) status = -4;
@@ -238,35 +272,33 @@ __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs
     const int all_n = scan_w[0][31], all_need = scan_w[1][31], all_gone = scan_w[2][31];
     __syncthreads();
     const int live = min(kPlanThreads, a.requests - r0);
-    // place e behind `from` in the ring; from is below twice its size, e below it
-    auto in_ring = [&](long long from, int e) {
-      long long p = from + e;
+    if (tid == 0) {
+      sh_need[live] = all_need;
+      sh_gone[live] = all_gone;
+      sh_rows[live] = base_n + all_n;
+    }
+    __syncthreads();
+    auto in_ring = [&](long long p) {  // p is below three times the ring's size
       while (p >= a.ring_size) p -= a.ring_size;
       return static_cast<int>(p);
     };
-    for (int e = tid; e < all_need; e += kPlanThreads * kPlanBatch) {
-      int i[kPlanBatch], id[kPlanBatch];
-#pragma unroll
-      for (int k = 0; k < kPlanBatch; ++k)
-        if (e + k * kPlanThreads < all_need)
-          id[k] = a.ring[in_ring(static_cast<long long>(head) + base_need, e + k * kPlanThreads)];
-      plan_find_batch(sh_need, live, e, kPlanThreads, i);
-#pragma unroll
-      for (int k = 0; k < kPlanBatch; ++k)
-        if (e + k * kPlanThreads < all_need)
-          a.tables[(r0 + i[k]) * a.ld_tables + sh_held[i[k]] + (e + k * kPlanThreads - sh_need[i[k]])] = id[k];
+    const long long from = static_cast<long long>(head) + base_need;
+    const long long to = static_cast<long long>(head) + available + base_gone;
+    plan_for_each(sh_need, live, big, [&](int i, int k) { return a.ring[in_ring(from + sh_need[i] + k)]; },
+                  [&](int i, int k, int id) { a.tables[(r0 + i) * a.ld_tables + sh_held[i] + k] = id; });
+    if (all_gone > 0) {
+      __syncthreads();  // big is free again
+      plan_for_each(sh_gone, live, big, [&](int i, int k) { return a.tables[(r0 + i) * a.ld_tables + k]; },
+                    [&](int i, int k, int id) { a.ring[in_ring(to + sh_gone[i] + k)] = id; });
     }
-    for (int e = tid; e < all_gone; e += kPlanThreads * kPlanBatch) {
-      int i[kPlanBatch], id[kPlanBatch];
-      plan_find_batch(sh_gone, live, e, kPlanThreads, i);
-#pragma unroll
-      for (int k = 0; k < kPlanBatch; ++k)
-        if (e + k * kPlanThreads < all_gone)
-          id[k] = a.tables[(r0 + i[k]) * a.ld_tables + (e + k * kPlanThreads - sh_gone[i[k]])];
-#pragma unroll
-      for (int k = 0; k < kPlanBatch; ++k)
-        if (e + k * kPlanThreads < all_gone)
-          a.ring[in_ring(static_cast<long long>(head) + available + base_gone, e + k * kPlanThreads)] = id[k];
+    if (a.fill_slots) {
+      __syncthreads();  // and the tables are whole
+      plan_for_each(sh_rows, live, big,
+                    [&](int i, int k) { return plan_slot(a, a.tables + (r0 + i) * a.ld_tables, a.start[r0 + i] + k); },
+                    [&](int i, int k, int slot) {
+                      a.slots[sh_rows[i] + k] = slot;
+                      a.positions[sh_rows[i] + k] = a.start[r0 + i] + k;
+                    });
     }
     base_n += all_n;
     base_need += all_need;
@@ -279,12 +311,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_cache_kernel(const PlanArgs
     a.ring_out[1] = available - base_need + base_gone;
     a.status[0] = 0;
   }
-  if (a.fill_slots) {
-    __syncthreads();
-    const int* first = a.requests <= kPlanThreads ? sh_rows : a.row_start;
-    for (int t = tid; t < a.max_rows; t += kPlanThreads * kPlanBatch)
-      plan_slots(a, first, base_n, t, kPlanThreads, a.max_rows);
-  }
+  if (a.fill_slots)
+    for (int t = base_n + tid; t < a.max_rows; t += kPlanThreads) a.slots[t] = a.positions[t] = -1;
 }
 
 // Slots and positions of a call with many rows, after plan_cache_kernel (programmatic dependent launch).
@@ -299,8 +327,28 @@ __global__ void __launch_bounds__(256) plan_slots_kernel(const PlanArgs a) {
     __syncthreads();
     first = sh;
   }
-  const int t = t0 + threadIdx.x, end = min(t0 + kPlanSlotRows, a.max_rows);
-  if (t < end) plan_slots(a, first, total, t, 256, end);
+  int r = 0;
+  bool found = false;
+  for (int t = t0 + threadIdx.x; t < min(t0 + kPlanSlotRows, a.max_rows); t += 256) {
+    if (t >= total) {
+      a.slots[t] = a.positions[t] = -1;
+      continue;
+    }
+    if (!found) {  // the first search over all requests, the next ones from there on
+      int hi = a.requests;
+      while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (first[mid] <= t) r = mid;
+        else hi = mid;
+      }
+      found = true;
+    } else {
+      r = plan_find(first, r, a.requests, t);
+    }
+    const int p = a.start[r] + (t - first[r]);
+    a.slots[t] = plan_slot(a, a.tables + r * a.ld_tables, p);
+    a.positions[t] = p;
+  }
 }
 
 // ---------------------------------------------------------------- append
