@@ -93,7 +93,9 @@ extern "C" int drt_cache_plan(const int32_t* start, const int32_t* count, const 
   a.max_rows = max_rows;
   a.lengths = lengths;
   a.status = status;
-  a.fill_slots = max_rows <= kPlanInlineRows;
+  // A token a request: the thread that plans a request writes its slot too (64 requests: 4.9 us in one launch, 6.2 in
+  // two). More: one CTA would write them all, so a second launch does (64 x 8 rows: 13.1 us in one, 7.4 in two).
+  a.fill_slots = max_rows <= requests;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   CK(launch(plan_cache_kernel, dim3(1), dim3(kPlanThreads), 0, st, false, a));
   if (!a.fill_slots)
@@ -196,8 +198,11 @@ extern "C" int drt_cache_read(const int32_t* slots, int32_t rows, const void* k_
 
 // ======================================================================= attention over the cache
 namespace {
-constexpr int kFewRows = 16;    // a row tile of the kernel for few rows
-constexpr int kManyRows = 48;   // average rows from which small requests ride along in the kernel for many
+// The kernel over few rows reads a unit's keys once for 8 or 16 rows, the one over many once for up to 256 but no
+// faster for one row than for 128. Rows of a kv head against us, 64 requests of 2,048 tokens in int8, 8 kv heads of 128:
+//   8: 64 (few), 177 (many)   16: 85, 184   32: 146, 185   64: 256, 190   128: 476, 200
+// and one request of 32,768 tokens: 25, 47   32, 49   43, 49   68, 50   119, 55.
+constexpr int kFewRows = 32;
 
 constexpr size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
@@ -322,14 +327,17 @@ extern "C" int drt_cache_attend(const drt_cache_attend_args* p, void* stream) {
   a.lse = p->lse;
   a.vec = aligned16(p->q) && (p->q_row | p->q_head) % 8 == 0;
   a.out_vec = aligned16(p->out) && (p->out_row | p->out_head) % 8 == 0;
-  // Rows of one kv head in a request: up to kFewRows go to the kernel for few, the rest to the one for many. One launch
-  // where the caller's bound or the average says that the other would find (nearly) nothing; either serves any count.
+  // Rows of one kv head in a request: up to kFewRows go to the kernel for few, the rest to the one for many; either
+  // serves any count. One launch where the caller's bound leaves nothing to the other kernel, or where the average is
+  // so near the bound that no more than 3 requests in 8 can be small: a launch that finds nothing costs 9 us (32 requests
+  // of 8 tokens x 8 heads: 113 us in two, 104 in one), while 64 requests of 2,048 tokens, of which a half (a quarter)
+  // have one row and the rest 64, take 313 us in two and 345 in one (with a quarter of one row and the rest 16: 197, 196).
   CacheAttnArgs b = a;
   attend_scratch(sms, p->dim, static_cast<uint8_t*>(p->scratch), &a, &b);
   const int max_rows = p->max_rows > 0 ? std::min(p->max_rows, p->q_rows) : p->q_rows;
   const int64_t rows = static_cast<int64_t>(max_rows) * a.group;
   const int64_t average = static_cast<int64_t>(p->q_rows) * a.group / p->requests;
-  const bool only_few = rows <= kFewRows, only_many = !only_few && average >= kManyRows;
+  const bool only_few = rows <= kFewRows, only_many = !only_few && average * 8 >= rows * 5;
   a.rows_from = only_many ? 1 : 0;
   a.rows_to = only_many ? 0 : only_few ? INT32_MAX : kFewRows;
   b.rows_from = only_few ? 1 : only_many ? 0 : kFewRows + 1;

@@ -74,7 +74,6 @@ __device__ __forceinline__ __nv_bfloat16 cache_out<__nv_bfloat16>(float x) { ret
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSlotRows = 1024;   // rows per CTA of 256 threads of plan_slots_kernel
 constexpr int kPlanStageRequests = 4096;  // row starts that a CTA keeps in shared memory
-constexpr int kPlanInlineRows = 4096;  // up to here the first kernel writes the slots itself: one launch
 
 struct PlanArgs {
   const int *start, *count, *held_in;

@@ -108,6 +108,15 @@ def test_plan_many_requests_and_rows(kernels):
     check_plan(kernels, *state, 16, rows + 3)
 
 
+def test_plan_uneven_requests(kernels):
+    """Fewer rows than requests, nearly all of them one request's, as one launch writes them."""
+    start, count, held, tables, ring, state, _ = serving_state(12, 900, 16, 0, 40, 0.1, spare=200)
+    tables = [row + [-1] * 45 for row in tables]
+    count[17], count[400], count[880] = 600, 33, 1
+    for max_rows in (634, 900, 901):
+        check_plan(kernels, start, count, held, tables, ring, state, 16, max_rows)
+
+
 def test_plan_without_requests(kernels):
     check_plan(kernels, [], [], [], [], [3, 4], [1, 2], 16, 3)
 
@@ -414,6 +423,16 @@ def test_attend_many_rows(kernels, mask_block, dim, code, typ):
     """Windows and prompt chunks beside single tokens."""
     requests = [(150, 190), (1, 70), (64, 64), (32, 333), (0, 5), (17, 400)]
     check_attend(kernels, attend_case(16, requests, 6, 2, dim, 32, code, typ, pad=4), mask_block)
+
+
+@pytest.mark.parametrize("dim,code,typ", [(128, I8, BF), (64, E4, HF)])
+def test_attend_rows_about_the_limit_between_the_kernels(kernels, dim, code, typ):
+    """31 to 33 rows of a kv head, bounds that leave one kernel out, and a small request among large ones."""
+    for heads, requests in ((8, [(8, 300), (5, 77), (8, 2000), (1, 64)]), (11, [(3, 300), (3, 1500)]), (31, [(1, 700), (1, 9)])):
+        case = attend_case(23, requests, heads, 1 if heads > 8 else 2, dim, 64, code, typ)
+        for bound in (0, max(n for n, _ in requests)):
+            check_attend(kernels, case, max_rows=bound)
+    check_attend(kernels, attend_case(24, [(32, 900), (32, 1290), (4, 70), (32, 333)], 8, 2, dim, 64, code, typ), 32, max_rows=32)
 
 
 @pytest.mark.parametrize("dim,code,typ,heads,kv_heads", [(128, E4, BF, 4, 2), (64, I8, HF, 3, 1), (128, I8, HF, 2, 2)])
