@@ -136,9 +136,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // keys serve all of its query heads) and it computes the transposed products on mma.sync m16n8k16,
 //   S^T [keys x rows] = K Q^T,   O^T [dims x rows] += V^T W^T,
 // with the codes as the 16-row operand: eight rows, the query heads of one token in a GQA model, then waste
-// nothing, and each code is expanded to f16 once, in the registers of the lane that read it. With so few rows the
-// tiles are bound by their bytes (256 B per key and head against 512 kNT MACs a byte pair needs); tcgen05 would
-// need the expanded codes written to shared memory first.
+// nothing, and each code is expanded to f16 once, in the registers of the lane that read it. A key costs 2 kDim bytes
+// and 16 kNT kDim multiply-adds, 8 kNT a byte, far below what the SM's mma.sync can do at the memory's rate, so the
+// bytes bound a long call; tcgen05 would need the expanded codes written to shared memory first.
+// Measured (dim 128): 64 requests of 8,192 tokens, 8 kv heads, 1.07 GB of codes: 176 us for 2 query heads each, 188 for
+// 8 (6.1 and 5.7 TB/s); 16 of 65,536, 4 kv heads of 7: 184 us. A start costs about 5 us (lengths, shares, first
+// tiles), the join in the CTA 3, the join's launch 4: one request of 130,001 tokens, 133 MB, takes 39 us (3.4 TB/s), one
+// of 4,096 tokens 16. Twelve warps to a CTA with two tiles in flight each were slower than eight with three.
 //
 // Lanes (g = lane / 4, q = lane % 4). The contracted index may be taken in any order that both operands share:
 //   K: a lane reads 16 bytes of a key's row, dimensions 16 (q + 4 half) .., four k-steps' worth of its fragment;
@@ -157,12 +161,12 @@ constexpr int kQrMaxRequests = 16384;
 template <int kDim, int kNT>
 struct QrCfg {
   static constexpr int kRows = 8 * kNT;
-  static constexpr int kWarps = kNT == 1 ? 8 : 8;
+  static constexpr int kWarps = 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kGroupBytes = 16 * kDim;
   static constexpr int kGroupPitch = kGroupBytes + 32;  // V reads of the four groups fall into different banks
   static constexpr int kSlot = 4 * kGroupPitch;
-  static constexpr int kSlots = (kWarps <= 8 ? 3 : 2) * (128 / kDim);
+  static constexpr int kSlots = 3 * (128 / kDim);
   static constexpr int kRing = kSlots * kSlot;
   static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kRing + kWarps * kSlots * 8;
 };
@@ -802,6 +806,7 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
 // Joins the parts of the units that CTAs' shares cut: the CTA in which a unit begins names it (tail part), its later
 // parts are the front parts of the CTAs up to the last. CTA (four owners, rows of the tile): a warp joins a unit of up
 // to kQmAlone parts, the whole CTA the longer ones, their parts dealt to the warps; either order is fixed by the shares.
+// Bound by the latency of three dependent reads (owner, statistics, parts): about 4 us after the rows kernel.
 constexpr int kQmThreads = 128;  // with their registers they fit beside a CTA of the rows kernel
 constexpr int kQmWarps = kQmThreads / 32;
 constexpr int kQmAlone = 4;

@@ -14,6 +14,10 @@
 // and stores the segment's maximum. Second kernel, one CTA per row: joins the slices' sums, and picks the
 // alternatives from the k segments with the largest maxima (equal maxima: the lowest segment). That those
 // segments hold all of them: a token outside has k segments whose largest token precedes it.
+//
+// Measured: 1,005 rows of 152,064 bf16 logits (306 MB) with 10 alternatives 80 us, 3.8 TB/s: 61 us for the first kernel,
+// bound by its instructions (69 % of the issue slots, 64 % of the exponentials' unit, 57 % of DRAM), 19 for the second,
+// which reads ten segments of each row again. 32 rows of f32: 18 us, one row 10 to 11, launches and latency.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -27,7 +31,7 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpCtasPerSm = 4;
-constexpr int kLpMaxSliceSegs = 64; // per CTA
+constexpr int kLpMaxSliceSegs = 64;  // per CTA
 constexpr int kLpMaxSegs = 4096;   // segments per row: 4 million logits
 constexpr int kLpCands = 512;      // candidate list of the second kernel
 
@@ -357,7 +361,9 @@ __device__ __forceinline__ float lp_key_value(unsigned long long k) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-// Threads per row: a batch fills the GPU with small CTAs, a few rows want their segments read at once.
+// Threads per row: a batch fills the GPU with small CTAs, a few rows want their segments read at once. Both kernels, 151,936
+// bf16 logits, top 8, with 512 and with 128: 1 row 9.4 and 11.1 us, 148 rows 20.9 and 21.4, 296 rows 32.0 and 33.0, 592 rows
+// 52.0 and 48.9, 1,184 rows 97.7 and 87.0.
 constexpr int kLpFinFewRows = 296, kLpFinMany = 128, kLpFinFew = 512;
 
 template <typename T>
