@@ -358,9 +358,10 @@ __global__ void __launch_bounds__(256) plan_slots_kernel(const PlanArgs a) {
 //   amax = max |x| over the run (finite values), s = max(amax / Q, s_old if the run does not begin the block)
 //   code = rn(x / s); the block's other tokens become rn(code * (s_old / s)) when s has grown
 // A run that begins a block starts it anew: what the block held before is gone.
-// x / s is taken as x * rn(1 / s) (two roundings of 2^-24 each before the rounding onto 8 bits, so a code
-// differs from the quotient's only within 2^-22 of a tie); a scale below 2^-100 divides instead, since its
-// reciprocal leaves the range.
+// x / s is the f32 quotient, as a tie between two codes is common (amax is a number of few bits, and so is half of it):
+// x * rn(1 / s) corrected by its residual (Markstein 1990), whose error before the last rounding is below 2^-46 of it. A
+// plain product moved 1.6 times as many ties to the other code. Scales outside [2^-100, 2^126], whose reciprocal or
+// residual would leave the range, and runs with infinities or NaN, divide.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendGroup = 32;  // rows whose runs a CTA looks for when the call has many, a lane each
 // Up to here eight rows to a CTA, a warp each if they are runs of their own, so that a step of single tokens fills the GPU:
@@ -380,9 +381,8 @@ struct AppendArgs {
   int vec;         // every row of k and v starts on a 16-byte boundary
 };
 
-// Four finite products |v| <= Q (1 + 2^-22) as codes. int8: adding 1.5 2^23 rounds to an integer (ties to even) in the
-// low byte, and none leaves [-127, 127]. (The callers' products are __fmul_rn: fused with this addition they would be
-// rounded once instead of twice.)
+// Four finite quotients |v| <= Q (1 + 2^-23) as codes. int8: adding 1.5 2^23 rounds to an integer (ties to even) in the
+// low byte, and none leaves [-127, 127].
 template <int kCode>
 __device__ __forceinline__ uint32_t finite_codes4(float v0, float v1, float v2, float v3) {
   if constexpr (kCode == CACHE_INT8) {
@@ -406,6 +406,12 @@ __device__ __forceinline__ uint32_t pair_max(uint32_t m, uint32_t x, __nv_bfloat
   const __nv_bfloat162 r =
       __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&m), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x)));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// x / s from inv = rn(1 / s). The signs keep a zero's own.
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+  const float q = __fmul_rn(x, inv);
+  return __fmaf_rn(__fmaf_rn(s, q, -x), -inv, q);
 }
 
 // A run of one or two rows by one warp, as single tokens of many requests are: eight values a lane. V's codes are
@@ -439,9 +445,7 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, const T* x, int6
 #pragma unroll
   for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
   const float s = fmaxf(__fdiv_rn(amax, code_max<kCode>()), s_old);
-  const bool divide = s > 0.0f && s < 0x1p-100f;
-  const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-  auto quant = [&](float y) { return divide ? __fdiv_rn(y, s) : s > 0.0f ? __fmul_rn(y, inv) : 0.0f; };
+  auto quant = [&](float y) { return s > 0.0f ? __fdiv_rn(y, s) : 0.0f; };
   uint8_t* dst = (is_v ? a.v_cache : a.k_cache) + at * (static_cast<int64_t>(a.block) * kDim);
   if (off > 0 && s > s_old) {  // every code of the block under the new scale; the run's own follow
     const float ratio = __fdiv_rn(s_old, s);
@@ -475,8 +479,8 @@ __device__ __forceinline__ void append_few(const AppendArgs& a, const T* x, int6
 
 // A longer run by the CTA. Its rows are read once, eight values a thread and turn: K's stay in registers until the scale is
 // known, V's go to shared memory and are read back by columns, two dimensions of 16 tokens a thread. Runs with an infinity
-// or a NaN, or with a scale below 2^-100, take the checked conversions; the other ones (about five instructions a value)
-// need none. Measured: two prompts of 14,500 rows together, 4 heads of 128, 45 MB read and written: 22 us (2.0 TB/s), bound
+// or a NaN, or with a scale outside the range above, take the checked conversions; the other ones (seven instructions a value)
+// need none. Measured: two prompts of 14,500 rows together, 4 heads of 128, 45 MB read and written: 23 us (1.9 TB/s), bound
 // by its instructions and the waits between reading and converting (56 % of the issue slots); 64 single tokens of 8 heads 5.
 template <typename T, int kDim, int kCode>
 __global__ void __launch_bounds__(kAppendThreads) append_cache_kernel(const AppendArgs a) {
@@ -582,13 +586,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_cache_kernel(const Appe
     const float s = fmaxf(__fdiv_rn(amax, code_max<kCode>()), s_old);
     const bool grew = off > 0 && s > s_old;
     const float ratio = grew ? __fdiv_rn(s_old, s) : 1.0f;
-    const bool divide = s > 0.0f && s < 0x1p-100f;
-    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-    const bool plain = finite && !divide;
-    auto checked4 = [&](float v0, float v1, float v2, float v3) {  // of products already taken
+    const bool plain = finite && s >= 0x1p-100f && s <= 0x1p126f;
+    const float inv = plain ? __fdiv_rn(1.0f, s) : 0.0f;
+    auto fast4 = [&](float v0, float v1, float v2, float v3) {
+      return finite_codes4<kCode>(quotient(v0, s, inv), quotient(v1, s, inv), quotient(v2, s, inv), quotient(v3, s, inv));
+    };
+    auto checked4 = [&](float v0, float v1, float v2, float v3) {  // of quotients already taken
       return f32_to_codes<kCode>(v0, v1) | f32_to_codes<kCode>(v2, v3) << 16;
     };
-    auto quant = [&](float v) { return divide ? __fdiv_rn(v, s) : s > 0.0f ? __fmul_rn(v, inv) : 0.0f; };
+    auto quant = [&](float v) { return s > 0.0f ? __fdiv_rn(v, s) : 0.0f; };
     auto again4 = [&](uint32_t w) {  // four codes of the block's other tokens under the new scale
       const float2 p = codes_to_f32<kCode>(w & 0xffffu), q2 = codes_to_f32<kCode>(w >> 16);
       return checked4(p.x * ratio, p.y * ratio, q2.x * ratio, q2.y * ratio);
@@ -603,8 +609,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_cache_kernel(const Appe
         const float2 p2 = pair_f32(mine[u].z, T()), p3 = pair_f32(mine[u].w, T());
         uint2 w;
         if (plain) {
-          w.x = finite_codes4<kCode>(__fmul_rn(p0.x, inv), __fmul_rn(p0.y, inv), __fmul_rn(p1.x, inv), __fmul_rn(p1.y, inv));
-          w.y = finite_codes4<kCode>(__fmul_rn(p2.x, inv), __fmul_rn(p2.y, inv), __fmul_rn(p3.x, inv), __fmul_rn(p3.y, inv));
+          w.x = fast4(p0.x, p0.y, p1.x, p1.y);
+          w.y = fast4(p2.x, p2.y, p3.x, p3.y);
         } else {
           w.x = checked4(quant(p0.x), quant(p0.y), quant(p1.x), quant(p1.y));
           w.y = checked4(quant(p2.x), quant(p2.y), quant(p3.x), quant(p3.y));
@@ -633,8 +639,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_cache_kernel(const Appe
             float2 v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = pair_f32(*reinterpret_cast<const uint32_t*>(e + (j * 4 + k) * kPitch), T());
-            w[0][j] = finite_codes4<kCode>(__fmul_rn(v[0].x, inv), __fmul_rn(v[1].x, inv), __fmul_rn(v[2].x, inv), __fmul_rn(v[3].x, inv));
-            w[1][j] = finite_codes4<kCode>(__fmul_rn(v[0].y, inv), __fmul_rn(v[1].y, inv), __fmul_rn(v[2].y, inv), __fmul_rn(v[3].y, inv));
+            w[0][j] = fast4(v[0].x, v[1].x, v[2].x, v[3].x);
+            w[1][j] = fast4(v[0].y, v[1].y, v[2].y, v[3].y);
           }
         } else {
           const uint4 o0 = p[0], o1 = p[1];

@@ -67,7 +67,7 @@ def token_major(cache, is_v):
 
 
 def append(x, slots, cache, scale, is_v):
-    """Rows x [rows, heads, dim] into copies of cache and scale, with the operator's own f32 steps: codes equal bit for bit."""
+    """Rows x [rows, heads, dim] into copies of cache and scale, in f32 steps: codes equal bit for bit."""
     dtype = cache.dtype
     held, scale = token_major(cache, is_v).clone(), scale.clone()
     block = held.shape[2]
@@ -88,12 +88,7 @@ def append(x, slots, cache, scale, is_v):
             s = torch.maximum(amax / QMAX[dtype], old)
             if off > 0 and s > old:
                 held[b, h] = to_code(held[b, h] * (old / s), dtype).float()
-            if s == 0:
-                codes = torch.zeros_like(rows)
-            elif s < 2.0 ** -100:
-                codes = rows / s
-            else:
-                codes = rows * (1.0 / s)
+            codes = torch.zeros_like(rows) if s == 0 else rows / s
             held[b, h, off:off + m] = to_code(codes, dtype).float()
             scale[b, h] = s
         t += m

@@ -180,8 +180,27 @@ def test_append(kernels, code, heads, block, dim, typ, runs):
     check_append(kernels, cache, k.to(typ), v.to(typ), slots)
 
 
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("typ", [BF, HF])
+def test_append_ties(kernels, code, typ):
+    """Values between two codes: the f32 quotient decides, over 2,400 (block, head) scales of many sizes; zeros keep their signs."""
+    block, heads, blocks = 16, 4, 300
+    g = torch.Generator().manual_seed(7)
+    cache = random_cache(7, blocks, heads, block, 64, code)
+
+    def rows():
+        top = torch.exp2(torch.rand(blocks, 1, heads, 1, generator=g) * 24 - 14).to(typ).float()  # of each block and head
+        step = torch.randint(-254, 255, (blocks, block, heads, 64), generator=g).float()
+        step[:, 3, :, 5] = 254
+        x = (top * step / 254).to(typ)
+        x[:, 7, :, 9] = -0.0
+        return x.reshape(blocks * block, heads, 64)
+
+    check_append(kernels, cache, rows(), rows(), list(range(blocks * block)))
+
+
 def test_append_many_rows_and_skipped_slots(kernels):
-    """Over 1024 rows a CTA looks for runs in 16 rows; slots of -1 and beyond the cache split runs and write nothing."""
+    """Over 1024 rows a CTA looks for runs in 32 rows; slots of -1 and beyond the cache split runs and write nothing."""
     block, blocks = 32, 50
     cache = random_cache(1, blocks, 2, block, 64, I8)
     order = list(range(blocks))
