@@ -169,6 +169,7 @@ struct QrCfg {
   static constexpr int kSlots = 3 * (128 / kDim);
   static constexpr int kRing = kSlots * kSlot;
   static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kRing + kWarps * kSlots * 8;
+  static_assert(kWarps * kRing >= (kQrMaxRequests + 1) * 8, "the requests' places stand in the rings' memory first");
 };
 constexpr int kQrMaxRows = 16;                 // of a tile
 constexpr int kQrMaxParts = 8 * 2 * kQrMaxRows;  // rows of the parts of a CTA's warps

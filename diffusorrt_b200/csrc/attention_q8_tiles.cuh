@@ -43,7 +43,8 @@ struct QtCfg {
   static constexpr int kStages = 2;                 // of K, of V, and of their codes together
   static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kCodes = kV + kStages * kTile;
   static constexpr int kEnd = kCodes + 2 * kRaw;
-  static constexpr size_t kSmem = 1024 + kEnd;     // tiles on 1024-byte boundaries
+  static constexpr int kPrefix = (kQrMaxRequests + 1) * 8;  // the requests' places, before the tiles need the memory
+  static constexpr size_t kSmem = 1024 + (kEnd > kPrefix ? kEnd : kPrefix);  // tiles on 1024-byte boundaries
 };
 
 struct __align__(16) QtMeta {

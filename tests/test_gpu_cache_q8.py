@@ -477,6 +477,40 @@ def test_attend_same_bits_again(kernels):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_most_requests(kernels, dim):
+    """16,384 requests, the most that a call takes: empty ones between single tokens and windows, by one kernel and by both."""
+    rng = random.Random(dim)
+    requests = [(0, 0)] * 16384
+    for r in rng.sample(range(16384), 60):
+        requests[r] = (rng.choice([1, 3]), rng.choice([5, 70, 300]))
+    for r in (0, 7001, 16383):
+        requests[r] = (40, 200)
+    case = attend_case(25, requests, 2, 1, dim, 64, I8, BF)
+    check_attend(kernels, case)
+    check_attend(kernels, attend_case(26, [(n if n < 9 else 1, m) for n, m in requests], 2, 1, dim, 64, E4, HF), max_rows=3)
+
+
+def test_blocks_beyond_four_gigabytes(kernels):
+    """The same rows through the first and the last blocks of a cache whose codes pass 32-bit offsets: the same bits."""
+    heads, block, dim, blocks = 8, 128, 128, 35_000  # 4.6 GB each of K and V
+    cache = kernels.cache_q8(blocks, heads, block, dim, dtype=I8)
+    g = torch.Generator().manual_seed(8)
+    k, v, q = (torch.randn(300, n, dim, generator=g).to(BF).cuda() for n in (heads, heads, 2 * heads))
+    got = []
+    for ids in ([0, 1, 2], [blocks - 1, blocks - 3, blocks - 2]):
+        slots = torch.cat([torch.arange(block) + b * block for b in ids])[:300].to(torch.int32).cuda()
+        kernels.append_cache_q8(k, v, slots, *cache)
+        back = kernels.read_cache_q8(slots, *cache)
+        tables, lengths = ints([ids]), ints([300])
+        many = kernels.attend_cache_q8(q, *cache, tables, lengths, ints([0, 300]))
+        few = kernels.attend_cache_q8(q[-2:], *cache, tables, lengths, ints([0, 2]), max_rows=2)
+        got.append((*back, *many, *few))
+    assert float(got[0][0].abs().max()) > 1
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_attend_nothing(kernels):
     q, cache, tables, lengths, starts = attend_case(19, [(1, 5)], 2, 2, 64, 16, I8, BF)
     out, lse = kernels.attend_cache_q8(q.cuda()[:0], *cuda(*cache), ints(tables), ints(lengths), ints([0, 0]))
