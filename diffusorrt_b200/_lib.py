@@ -184,7 +184,7 @@ SIGNATURES = {
     "drt_cache_attend_scratch_bytes": (ctypes.c_size_t, [_I32]),
     "drt_cache_attend": (ctypes.c_int, [_P, _P]),  # the address or bytes of a CacheAttendArgs
     "drt_selector_logprobs_scratch_bytes": (ctypes.c_size_t, [_I32, _I32, _I32]),
-    "drt_selector_logprobs": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I32, _P, ctypes.c_double, _I32, _I32, _P, _P, _P,
+    "drt_selector_logprobs": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _I32, _I32, _P, ctypes.c_double, _I32, _I32, _P, _P, _P,
                                              _P, _P, _P, _P]),
     "drt_linear_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     "drt_linear_bf16": (ctypes.c_int, [_P, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,

@@ -386,11 +386,12 @@ extern "C" size_t drt_selector_logprobs_scratch_bytes(int32_t rows, int32_t voca
   return up256(static_cast<size_t>(rows) * p.slices * 16) + up256(static_cast<size_t>(rows) * p.segs * 4);
 }
 
-extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, const int32_t* row_index, int32_t rows,
-                                     int32_t vocab, const int32_t* tokens, double temperature, int32_t exclude_token,
-                                     int32_t top, void* scratch, float* logprob, float* entropy, int32_t* rank,
-                                     int32_t* top_token, float* top_logprob, void* stream) {
+extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t logit_rows,
+                                     const int32_t* row_index, int32_t rows, int32_t vocab, const int32_t* tokens,
+                                     double temperature, int32_t exclude_token, int32_t top, void* scratch, float* logprob,
+                                     float* entropy, int32_t* rank, int32_t* top_token, float* top_logprob, void* stream) {
   REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab, "bad selector geometry");
+  REQUIRE(logit_rows >= (row_index ? 1 : rows) || rows == 0, "more rows than logits");
   REQUIRE(dtype == DRT_TYPE_F32 || dtype == DRT_TYPE_BF16 || dtype == DRT_TYPE_F16, "logits must be f32, bf16 or f16");
   REQUIRE(top >= 0 && top <= kLpMaxTop, "top must be in [0, %d]", kLpMaxTop);
   REQUIRE(std::isfinite(temperature) && (temperature <= 0.0 || temperature >= 1e-30),
@@ -414,6 +415,7 @@ extern "C" int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t 
   a.row_index = row_index;
   a.tokens = tokens;
   a.rows = rows;
+  a.logit_rows = logit_rows;
   a.vocab = vocab;
   a.top = top;
   a.exclude = exclude_token;

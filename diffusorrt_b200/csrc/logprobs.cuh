@@ -42,7 +42,7 @@ struct LogprobArgs {
   int64_t ld;
   const int* row_index;
   const int* tokens;
-  int rows, vocab, top, exclude;
+  int rows, logit_rows, vocab, top, exclude;
   float unit_log2;       // c
   int segs, slices, segs_per_slice;
   // scratch
@@ -213,6 +213,15 @@ __device__ __forceinline__ uint4 lp_pick(const uint4* u, int v) {
   return w;
 }
 
+// Row r of the call and its logits: none for an index outside them.
+template <typename T>
+__device__ __forceinline__ const T* lp_row(const LogprobArgs& a, int r, int& vocab) {
+  const int at = a.row_index ? a.row_index[r] : r;
+  const bool there = at >= 0 && at < a.logit_rows;
+  vocab = there ? a.vocab : 0;
+  return static_cast<const T*>(a.logits) + (there ? at : 0) * a.ld;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_stats_kernel(const LogprobArgs a) {
   using Seg = LpSeg<T>;
@@ -220,10 +229,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_stats_kernel
   __shared__ float4 warp_part[kLpWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-  const T* row = static_cast<const T*>(a.logits) + static_cast<int64_t>(a.row_index ? a.row_index[r] : r) * a.ld;
+  int vocab;
+  const T* row = lp_row<T>(a, r, vocab);
   const int off = lp_offset(row);
   const int t = a.tokens ? a.tokens[r] : -1;
-  const bool given = t >= 0 && t < a.vocab;
+  const bool given = t >= 0 && t < vocab;
   const float xt = !given || t == a.exclude ? -INFINITY : lp_f32(row[t]);
   const float c = a.unit_log2;
   const bool low_token = xt == -INFINITY;
@@ -233,7 +243,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) logprob_stats_kernel
   const int seg1 = min((slice + 1) * a.segs_per_slice, a.segs);
   for (int seg = slice * a.segs_per_slice + warp; seg < seg1; seg += kLpWarps) {
     uint4 u[8];
-    Seg::load(row, off, a.vocab, a.exclude, seg, lane, u);
+    Seg::load(row, off, vocab, a.exclude, seg, lane, u);
     const float bm = Type::largest(u, 8);
     if (a.rank && bm >= xt) {  // else nothing of this lane's precedes the token
       const int at = seg * Seg::kSeg - off;  // token of the segment's first position
@@ -380,7 +390,8 @@ __global__ void __launch_bounds__(kLpFinFew, 2) logprob_finish_kernel(const Logp
   __shared__ unsigned long long best[kLpFinFew / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads / 32;
   const int r = blockIdx.x;
-  const T* row = static_cast<const T*>(a.logits) + static_cast<int64_t>(a.row_index ? a.row_index[r] : r) * a.ld;
+  int vocab;
+  const T* row = lp_row<T>(a, r, vocab);
   const int off = lp_offset(row);
   if (tid < kLpMaxTop) picked[tid] = -1;
   if (tid == 0) {
@@ -422,7 +433,7 @@ __global__ void __launch_bounds__(kLpFinFew, 2) logprob_finish_kernel(const Logp
     }
     if (lane == 0) {
       const int t = a.tokens ? a.tokens[r] : -1;
-      const bool given = t >= 0 && t < a.vocab;
+      const bool given = t >= 0 && t < vocab;
       const float xt = !given || t == a.exclude ? -INFINITY : lp_f32(row[t]);
       constexpr double kLn2 = 0.69314718055994530942;
       const double ls = log(S), R = ref(m);
@@ -451,7 +462,7 @@ __global__ void __launch_bounds__(kLpFinFew, 2) logprob_finish_kernel(const Logp
   const float low = cut;
   auto offer = [&](int seg, auto&& f) {  // f(key) for this lane's tokens of `seg` that may be listed
     uint4 u[8];
-    Seg::load(row, off, a.vocab, a.exclude, seg, lane, u);
+    Seg::load(row, off, vocab, a.exclude, seg, lane, u);
     uint32_t hit = 0;                    // the vectors that hold one: few
 #pragma unroll
     for (int v = 0; v < 8; ++v) hit |= (Type::largest(u + v, 1) >= low) << v;
@@ -459,7 +470,7 @@ __global__ void __launch_bounds__(kLpFinFew, 2) logprob_finish_kernel(const Logp
       const int v = __ffs(hit) - 1, tok = seg * Seg::kSeg - off + (v * 32 + lane) * Seg::kVec;
 #pragma unroll 1
       for (int i = 0; i < Seg::kVec; ++i) {
-        if (tok + i < 0 || tok + i >= a.vocab || tok + i == a.exclude) continue;
+        if (tok + i < 0 || tok + i >= vocab || tok + i == a.exclude) continue;
         const float x = lp_f32(row[tok + i]);
         if (x >= low && x > -INFINITY) f(lp_key(x, tok + i));
       }

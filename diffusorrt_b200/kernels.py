@@ -458,6 +458,8 @@ def attend_cache_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif not (isinstance(lse, torch.Tensor) and lse.dtype is torch.float32 and lse.get_device() == index
               and lse.shape == (rows, heads) and lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [rows, heads] tensor")
+    if not (0 <= mask_block <= 1 << 24 and 0 <= max_rows < 1 << 31):
+        raise ValueError("mask_block outside [0, 2^24] or max_rows outside [0, 2^31)")
     size = _attend_bytes(dim, index)
     if scratch is None:
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
@@ -494,7 +496,8 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
                     stream: torch.cuda.Stream | None = None) -> TokenScores:
     """Log probabilities of given tokens (int32) under softmax(logits / T) of f32, bf16 or f16 rows [rows, vocab]
     (or of the rows row_index), with the entropy, the token's rank and the `top` <= 32 likeliest tokens.
-    exclude_token counts as a logit of -inf; a token outside the vocabulary scores -inf with rank -1."""
+    exclude_token counts as a logit of -inf; a token outside the vocabulary, or of a row_index
+    outside the logits, scores -inf with rank -1."""
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2):
         raise ValueError("logits must be a CUDA tensor [rows, vocab]")
     index = logits.get_device()
@@ -511,6 +514,8 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
         raise ValueError("one token per logits row")
     if not 0 <= top <= 32:
         raise ValueError("top must be in [0, 32]")
+    if not -1 <= exclude_token < vocab:
+        raise ValueError("exclude_token outside the vocabulary")
     size = _logprob_bytes(n, vocab, typ, index)
     words = n * (3 + 2 * top)
     # outputs in one allocation, the call's scratch in front of them
@@ -524,7 +529,7 @@ def select_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     p = made.data_ptr()
     at = p + 4 * own
     _launch(index, stream, (made,) if scratch is None else (made, scratch), _lib.load().drt_selector_logprobs,
-            logits.data_ptr(), typ, max(ld, vocab), 0 if row_index is None else row_index.data_ptr(), n, vocab,
+            logits.data_ptr(), typ, max(ld, vocab), have, 0 if row_index is None else row_index.data_ptr(), n, vocab,
             tokens.data_ptr(), temperature, exclude_token, top, p if scratch is None else scratch.data_ptr(), at, at + 4 * n,
             at + 4 * n * (2 + top), at + 4 * n * (3 + top), at + 8 * n)
     return TokenScores(logprob, entropy, rank, top_token.view(n, top), top_logprob.view(n, top))

@@ -433,16 +433,16 @@ typedef struct drt_cache_attend_args {
 size_t drt_cache_attend_scratch_bytes(int32_t dim);
 int drt_cache_attend(const drt_cache_attend_args* args, void* stream);
 /* Scores of given tokens under softmax(x / T) (T <= 0: no scaling, else T >= 1e-30) of rows of logits (DRT_TYPE_*, row r or
- * row_index[r], row stride ld): logprob[r] of tokens[r] (-inf for a token outside the vocabulary, whose rank
+ * row_index[r], of logit_rows rows with stride ld): logprob[r] of tokens[r] (-inf for a token outside the vocabulary, whose rank
  * is -1), entropy[r] in nats, rank[r] = tokens before it by (logit, lowest id), and the `top` (at most 32)
  * likeliest tokens with their log probabilities in that order, -1 and -inf behind the last of non-zero
  * probability. exclude_token (-1: none) counts as -inf. A row without any finite or +inf logit gives -inf,
- * entropy 0 and no alternatives; a NaN in a row gives NaN log probabilities and entropy. Null outputs are
+ * entropy 0 and no alternatives, and so does a row_index outside the logits (rank -1); a NaN in a row gives NaN log probabilities and entropy. Null outputs are
  * left out. The selectors above score the argmax; this scores what was answered. */
 size_t drt_selector_logprobs_scratch_bytes(int32_t rows, int32_t vocab, int32_t dtype);
-int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, const int32_t* row_index, int32_t rows,
-                          int32_t vocab, const int32_t* tokens, double temperature, int32_t exclude_token, int32_t top,
-                          void* scratch, float* logprob, float* entropy, int32_t* rank, int32_t* top_token,
+int drt_selector_logprobs(const void* logits, int32_t dtype, int64_t ld, int32_t logit_rows, const int32_t* row_index,
+                          int32_t rows, int32_t vocab, const int32_t* tokens, double temperature, int32_t exclude_token,
+                          int32_t top, void* scratch, float* logprob, float* entropy, int32_t* rank, int32_t* top_token,
                           float* top_logprob, void* stream);
 /* y = x @ W^T on the tensor cores with the MLX rounding contract (bf16 output rounding when
  * round_bf16 != 0). x [rows x K] bf16, w [n x K] bf16, y [rows x n] f32; n % 128 == 0,

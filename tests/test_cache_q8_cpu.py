@@ -121,7 +121,7 @@ def test_attend_refusals(lib, change, message):
 
 
 def score(lib, **change):
-    a = dict(logits=P, dtype=0, ld=100, index=None, rows=2, vocab=100, tokens=P, temperature=0.0, exclude=-1, top=2, scratch=P, lp=P,
+    a = dict(logits=P, dtype=0, ld=100, logit_rows=2, index=None, rows=2, vocab=100, tokens=P, temperature=0.0, exclude=-1, top=2, scratch=P, lp=P,
              ent=P, rank=P, tt=P, tl=P)
     a.update(change)
     return lib.drt_selector_logprobs(*a.values(), None)
@@ -132,7 +132,7 @@ def score(lib, **change):
     (dict(dtype=5), "logits"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(temperature=float("inf")), "temperature"),
     (dict(temperature=1e-31), "temperature"),
     (dict(exclude=100), "exclude"), (dict(ld=99), "geometry"), (dict(vocab=0), "geometry"), (dict(rows=-1), "geometry"),
-    (dict(logits=P + 2), "misaligned")])
+    (dict(logits=P + 2), "misaligned"), (dict(logit_rows=1), "more rows"), (dict(logit_rows=0, index=P), "more rows")])
 def test_score_refusals(lib, change, message):
     refuse(lib, score(lib, **change), "score", message)
 

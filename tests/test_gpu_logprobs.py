@@ -96,6 +96,20 @@ def test_strides_and_row_index(kernels):
               row_index=torch.tensor(pick, dtype=torch.int32, device="cuda"))
 
 
+def test_row_index_outside_the_logits(kernels):
+    """Such a row reads nothing and scores nothing; its neighbours are as ever."""
+    x, tokens = rows(9, 3, 5000, torch.bfloat16)
+    index = torch.tensor([1, -1, 3, 2**31 - 1, 0], dtype=torch.int32, device="cuda")
+    given = torch.tensor([5, 6, 7, 8, tokens[0]], dtype=torch.int32, device="cuda")
+    p = kernels.select_logprobs(x.cuda(), given, top=3, row_index=index)
+    q = kernels.select_logprobs(x.cuda()[[1, 0]], given[[0, 4]], top=3)
+    for a, b in zip(p, q):
+        assert torch.equal(a[[0, 4]], b)
+    for r in (1, 2, 3):
+        assert p.logprob[r] == -math.inf and p.entropy[r] == 0 and p.rank[r] == -1
+        assert p.top_token[r].tolist() == [-1] * 3 and p.top_logprob[r].tolist() == [-math.inf] * 3
+
+
 def test_equal_logits(kernels):
     """More equal logits than the candidate list holds: the lowest ids win."""
     x = torch.zeros(3, 30000)
