@@ -805,16 +805,20 @@ __global__ void __launch_bounds__(QrCfg<kDim, kNT>::kThreads, 1) cache_attn_rows
 }
 
 // Joins the parts of the units that CTAs' shares cut: the CTA in which a unit begins names it (tail part), its later
-// parts are the front parts of the CTAs up to the last. CTA (four owners, rows of the tile): a warp joins a unit of up
-// to kQmAlone parts, the whole CTA the longer ones, their parts dealt to the warps; either order is fixed by the shares.
-// Bound by the latency of three dependent reads (owner, statistics, parts): about 4 us after the rows kernel.
+// parts are the front parts of the CTAs up to the last. CTA (four owners, `step` rows of the tile): half a warp joins a row
+// of a unit of up to kQmAlone parts, all of them read at once, the whole CTA a row of the longer ones, their parts dealt to
+// the warps; either order is fixed by the shares.
+// Bound by the latency of dependent reads (owner, then statistics, parts and the request's place): 2.5 to 6 us after the
+// kernel over few rows; 13 us after the one over many for two prompts, whose 148 cut units leave 40 MB. A warp to a row with
+// its parts read in turn took 1.3 and 6 us more; as many CTAs as are resident, each through several rows, 3 us more.
 constexpr int kQmThreads = 128;  // with their registers they fit beside a CTA of the rows kernel
 constexpr int kQmWarps = kQmThreads / 32;
 constexpr int kQmAlone = 4;
 
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const CacheAttnArgs a, int ctas) {
+__global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const CacheAttnArgs a, int ctas, int step) {
   constexpr int kE = kDim / 32;  // dimensions per lane
+  constexpr int kE2 = kDim / 16; // with half a warp to a row
   __shared__ float red[kQmWarps][kDim];
   __shared__ float red_s[kQmWarps];
   griddep_wait();
@@ -823,10 +827,52 @@ __global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const Cach
   int4 mine = make_int4(0, 0, 0, 0);  // lane i of every warp holds owner base + i
   if (lane < kQmWarps && base + lane < ctas) mine = a.desc[base + lane];
   const int my_parts = (mine.x >> 9) - (base + lane) + 1, my_rows = mine.x & 511;
-  for (int row = blockIdx.y; row < kRows; row += gridDim.y) {
+  for (int row = blockIdx.y * step; row < kRows; row += gridDim.y * step) {
     const uint32_t alone = __ballot_sync(~0u, row < my_rows && my_parts <= kQmAlone);
+    if (__ballot_sync(~0u, row < my_rows) == 0) break;  // later rows have no owner either
+    if (alone >> warp & 1) {
+      const int parts = __shfl_sync(~0u, my_parts, warp), rows = __shfl_sync(~0u, my_rows, warp);
+      const int r = __shfl_sync(~0u, mine.y, warp), t = __shfl_sync(~0u, mine.z, warp), h = __shfl_sync(~0u, mine.w, warp);
+      const int own = row + (lane >> 4), at_dim = (lane & 15) * kE2;
+      if ((lane >> 4) < step && own < rows) {
+        float4 s[kQmAlone];
+        float v[kQmAlone][kE2];
+#pragma unroll
+        for (int p = 0; p < kQmAlone; ++p) {
+          s[p] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+          if (p < parts) {
+            const int64_t at = (static_cast<int64_t>(base + warp + p) * 2 + (p == 0 ? 1 : 0)) * kRows + own;
+            s[p] = a.cta_stat[at];
+#pragma unroll
+            for (int e = 0; e < kE2; e += 4) qa_load<4>(v[p] + e, a.cta_part + at * kDim + at_dim + e);
+          }
+        }
+        float m = -INFINITY, M = -INFINITY, l = 0.0f, acc[kE2];
+#pragma unroll
+        for (int p = 0; p < kQmAlone; ++p) {
+          m = fmaxf(m, s[p].x);
+          M = fmaxf(M, s[p].y);
+        }
+        const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int e = 0; e < kE2; ++e) acc[e] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < kQmAlone; ++p) {
+          if (p >= parts) break;
+          const float f = qa_ex2(s[p].y - Z);
+          l += s[p].z * qa_ex2(s[p].x - z);
+#pragma unroll
+          for (int e = 0; e < kE2; ++e) acc[e] += v[p][e] * f;
+        }
+        qa_put<T, kE2>(a, r, t * kRows + own, h, lane & 15, z, Z, m, l, acc);
+      }
+      __syncwarp();
+    }
+  }
+  for (int first = blockIdx.y * step, k = 0; first + k < kRows; k + 1 < step ? ++k : (k = 0, first += gridDim.y * step)) {
+    const int row = first + k;
     uint32_t many = __ballot_sync(~0u, row < my_rows && my_parts > kQmAlone);
-    if ((alone | many) == 0) return;  // later rows have no owner either
+    if (many == 0) return;
     auto slot = [&](int c0, int p) { return (static_cast<int64_t>(c0 + p) * 2 + (p == 0 ? 1 : 0)) * kRows + row; };
     auto maxima = [&](int c0, int parts, int p0, int step, float& m, float& M) {
       for (int p = p0; p < parts; p += step) {
@@ -854,17 +900,6 @@ __global__ void __launch_bounds__(kQmThreads) cache_attn_merge_kernel(const Cach
         for (int e = 0; e < kE; ++e) acc[e] += part[e] * f;
       }
     };
-    if (alone >> warp & 1) {
-      const int parts = __shfl_sync(~0u, my_parts, warp);
-      float m = -INFINITY, M = -INFINITY, l = 0.0f, acc[kE];
-#pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
-      maxima(base + warp, parts, lane, 32, m, M);
-      const float z = m == -INFINITY ? 0.0f : m, Z = M == -INFINITY ? 0.0f : M;
-      add(base + warp, parts, 0, 1, z, Z, acc, l);
-      qa_put<T, kE>(a, __shfl_sync(~0u, mine.y, warp), __shfl_sync(~0u, mine.z, warp) * kRows + row,
-                    __shfl_sync(~0u, mine.w, warp), lane, z, Z, m, l, acc);
-    }
     for (; many; many &= many - 1) {
       const int i = __ffs(many) - 1;
       const int parts = __shfl_sync(~0u, my_parts, i);

@@ -14,7 +14,7 @@
 // memory 320 KB = 2500 clocks (codes in and out 128, Q and K operands 128, V 64): W stays in TMEM for that reason.
 // The references m and M of a row move only when they are off by more than 2^8 (weights then reach 256, far inside
 // f16), so O is rescaled a few times per unit and not once per tile.
-// Measured: two prompts of about 2,200 rows behind 5,500 tokens, 28 heads on 4, dim 128 (252 GFLOP): 358 us, 705 TFLOP/s;
+// Measured: two prompts of about 2,200 rows behind 5,500 tokens, 28 heads on 4, dim 128 (252 GFLOP): 352 us, 716 TFLOP/s;
 // the tensor pipe is busy 35 % of the time and the exponentials' unit 37 %. What bounds it is the chain of one row tile:
 // S out of TMEM, maximum, weights and W back (3.4 thousand clocks), then its products (1.8). 128 keys take 5.8 to 6.6
 // thousand clocks for one row tile and hardly more for two in turn, so units of at most 128 rows pay most: 8 windows of 32

@@ -231,9 +231,12 @@ size_t attend_scratch(int sms, int dim, uint8_t* base, CacheAttnArgs* few, Cache
 
 template <typename T, int kDim, int kRows>
 cudaError_t run_merge(const CacheAttnArgs& a, int grid, int64_t rows, cudaStream_t st) {
+  // two rows to a CTA where the units are so many that most have few parts, else one: a long unit takes the whole CTA
+  const int64_t units = (static_cast<int64_t>(a.q_rows) * a.group / kRows + a.requests) * a.heads;
+  const int step = units * kQmAlone >= grid ? 2 : 1;
   return launch(cache_attn_merge_kernel<T, kDim, kRows>,
-                dim3((grid + kQmWarps - 1) / kQmWarps, static_cast<unsigned>(std::min<int64_t>(rows, kRows))), dim3(kQmThreads), 0,
-                st, true, a, grid);
+                dim3((grid + kQmWarps - 1) / kQmWarps, static_cast<unsigned>((std::min<int64_t>(rows, kRows) + step - 1) / step)),
+                dim3(kQmThreads), 0, st, true, a, grid, step);
 }
 
 // rows: the most rows of one kv head's queries in a request; tiles: an upper bound on the key tiles of all units;
