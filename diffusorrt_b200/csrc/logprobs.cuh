@@ -459,7 +459,36 @@ __global__ void __launch_bounds__(kLpFinFew, 2) logprob_finish_kernel(const Logp
   }
   if (a.top == 0) return;
   __syncthreads();
-  const float low = cut;
+  float low = cut;
+  if (low == -INFINITY) {
+    // fewer segments than alternatives, and their maxima bound nothing: the `top`-th largest of the maxima of 32 / width
+    // lanes' tokens does (at least two maxima for each alternative, if there are enough lanes). 1,005 rows of 32,000 bf16
+    // logits with 20 alternatives: 52 us; without a bound every token was a candidate, 1,163 us.
+    float* part_max = reinterpret_cast<float*>(cand);  // at most kLpMaxTop * 32
+    const int n_seg = min(a.top, a.segs);
+    int width = 32;                                    // lanes to a maximum
+    while (width > 1 && n_seg * (32 / width) < 2 * a.top) width >>= 1;
+    const int n_max = n_seg * (32 / width);
+    for (int p = warp; p < n_seg; p += warps) {
+      float v = -INFINITY;
+      if (picked[p] >= 0) {
+        uint4 u[8];
+        Seg::load(row, off, vocab, a.exclude, picked[p], lane, u);
+        v = Type::largest(u, 8);
+      }
+      for (int o = width >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+      if (lane % width == 0) part_max[p * (32 / width) + lane / width] = v;
+    }
+    __syncthreads();
+    for (int i = tid; i < n_max; i += threads) {
+      const float v = part_max[i];
+      int before = 0;
+      for (int q = 0; q < n_max; ++q) before += part_max[q] > v || (part_max[q] == v && q < i);
+      if (before == a.top - 1) cut = v;
+    }
+    __syncthreads();
+    low = cut;
+  }
   auto offer = [&](int seg, auto&& f) {  // f(key) for this lane's tokens of `seg` that may be listed
     uint4 u[8];
     Seg::load(row, off, vocab, a.exclude, seg, lane, u);
