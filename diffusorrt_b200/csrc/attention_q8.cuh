@@ -140,9 +140,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // and 16 kNT kDim multiply-adds, 8 kNT a byte, far below what the SM's mma.sync can do at the memory's rate, so the
 // bytes bound a long call; tcgen05 would need the expanded codes written to shared memory first.
 // Measured (dim 128): 64 requests of 8,192 tokens, 8 kv heads, 1.07 GB of codes: 176 us for 2 query heads each, 188 for
-// 8 (6.1 and 5.7 TB/s); 16 of 65,536, 4 kv heads of 7: 184 us. A start costs about 5 us (lengths, shares, first
+// 8 (6.1 and 5.7 TB/s); 16 of 65,536, 4 kv heads of 7: 174 us. A start costs about 5 us (lengths, shares, first
 // tiles), the join in the CTA 3, the join's launch 4: one request of 130,001 tokens, 133 MB, takes 39 us (3.4 TB/s), one
-// of 4,096 tokens 16. Twelve warps to a CTA with two tiles in flight each were slower than eight with three.
+// of 4,096 tokens 15. Twelve warps to a CTA with two tiles in flight each were slower than eight with three.
 //
 // Lanes (g = lane / 4, q = lane % 4). The contracted index may be taken in any order that both operands share:
 //   K: a lane reads 16 bytes of a key's row, dimensions 16 (q + 4 half) .., four k-steps' worth of its fragment;

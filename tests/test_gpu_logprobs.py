@@ -118,6 +118,24 @@ def test_equal_logits(kernels):
     check(kernels, x, [29999, 5, 4], 20)
 
 
+@pytest.mark.parametrize("typ", [torch.float32, torch.bfloat16])
+def test_fewer_segments_than_alternatives(kernels, typ):
+    """Rows whose alternatives are bounded by lanes' maxima: equal ones, all in one lane, hardly any, none."""
+    x, _ = rows(10, 7, 6001, typ)
+    x[0] = 0.5
+    x[1, 40:] = -math.inf
+    x[2] = -math.inf
+    x[3] = -5.0
+    x[3, 3000:3040] = torch.arange(40).to(typ) / 8
+    x[4, 1:] = -math.inf
+    x[5, ::2] = math.nan
+    x[5, 1::2] = 1.0
+    check(kernels, x[[0, 1, 2, 3, 4, 6]], [6000, 3, 5, 3001, 0, 17], 32, exclude=3002)
+    p = kernels.select_logprobs(x.cuda(), torch.zeros(7, dtype=torch.int32, device="cuda"), top=32)
+    # a NaN is no alternative
+    assert p.top_token[5].tolist() == list(range(1, 65, 2)) and bool(torch.isnan(p.logprob[5]))
+
+
 def test_masked_infinite_and_nan_logits(kernels):
     x, _ = rows(4, 8, 2500)
     x[0] = -math.inf                         # nothing can be drawn
